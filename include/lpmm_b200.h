@@ -461,6 +461,92 @@ int lpmm_b200_adamw4bit_factored_step_noalloc(const lpmm_b200_step_tensor* t, co
                                               double beta2, double lr, double weight_decay, double eps, double step,
                                               void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * Training losses with their gradients (no counterpart in the reference, whose step begins at p.grad).
+ * ------------------------------------------------------------------------------------------------ */
+#define LPMM_B200_DTYPE_FP32 0            /* beside LPMM_B200_DTYPE_BF16 and _FP16              */
+
+#define LPMM_B200_REDUCE_NONE 0           /* one loss per row                                  */
+#define LPMM_B200_REDUCE_SUM 1
+#define LPMM_B200_REDUCE_MEAN 2           /* sum / sum of the weights (0 if that is 0)         */
+
+#define LPMM_B200_DISTILL_MAX_K 1024      /* stored teacher logits per row                     */
+#define LPMM_B200_DISTILL_MIN_T 0.0009765625f
+#define LPMM_B200_DISTILL_MAX_T 1024.0f
+
+/* Distillation from a teacher's K stored top logits.  Per row, with the student's logits x over `vocab` columns, the
+ * teacher's logits t_k of the columns index_k and a temperature T:
+ *   p_k = exp(t_k/T) / sum_j exp(t_j/T),  q_v = exp(x_v/T) / sum_u exp(x_u/T),
+ *   loss = weight * T^2 * sum_k p_k (log p_k - log q_{index_k}),
+ *   d loss / d x_v = weight * T * (q_v - sum over k with index_k = v of p_k).
+ * A negative index or t_k = -inf is no entry.  A row of weight 0, or without entries, has loss 0 and gradient 0 and its
+ * logits are not looked at.  An index >= vocab makes its row's loss and gradient NaN; nothing out of range is accessed.
+ * Sums and statistics are fp32 (the sum over rows double), the gradient is rounded once; results do not depend on
+ * how the work is scheduled (no floating-point atomics). */
+typedef struct lpmm_b200_distill {
+  const void* logits;      /* row r begins at element (r / inner) * outer_stride + (r % inner) * inner_stride           */
+  void* grad;              /* [rows, vocab] contiguous, type of the logits (not for forward)                            */
+  const void* teacher;     /* [rows, k] contiguous, teacher_dtype                                                       */
+  const void* index;       /* [rows, k] contiguous, index_bits wide                                                     */
+  const float* weights;    /* [rows], or NULL for 1                                                                     */
+  const float* upstream;   /* backward only: derivative by the loss, one value, or [rows] with REDUCE_NONE              */
+  float* loss;             /* one value, or [rows] with REDUCE_NONE (not for backward)                                  */
+  float* work;             /* lpmm_b200_distill_work_floats(rows) floats, 16-byte aligned; forward leaves in it what    */
+                           /* backward reads                                                                            */
+  int64_t rows, inner, outer_stride, inner_stride;
+  int64_t vocab;
+  int64_t k;
+  int32_t dtype, teacher_dtype, index_bits, reduction;
+  float temperature;
+  float grad_scale;        /* factor of the gradient                                                                    */
+} lpmm_b200_distill;
+
+int64_t lpmm_b200_distill_work_floats(int64_t rows);
+int lpmm_b200_distill_forward(const lpmm_b200_distill* d, void* stream);
+/* upstream * grad_scale * gradient, from the `work` that forward left. */
+int lpmm_b200_distill_backward(const lpmm_b200_distill* d, void* stream);
+/* Loss, and grad_scale * the gradient of its sum over rows (REDUCE_NONE, _SUM) or of its mean, in one call. */
+int lpmm_b200_distill_forward_backward(const lpmm_b200_distill* d, void* stream);
+
+#define LPMM_B200_BALANCE_MAX_EXPERTS 1024
+#define LPMM_B200_SCORE_SOFTMAX 0
+#define LPMM_B200_SCORE_SIGMOID 1
+
+/* Load-balance loss of a router and the number of assignments per expert.  For the n valid tokens of a sequence, their
+ * scores p (softmax of the router's logits over the experts, or their sigmoids divided by the sigmoids' sum) and the
+ * k experts chosen for each token:
+ *   count_e = assignments to e,  f_e = experts * count_e / (k n),  P_e = mean of p_e,  loss = sum_e f_e P_e,
+ *   d loss / d x_e = experts / (k n^2) * p_e * (count_e - sum_j count_j p_j)   (times 1 - sigmoid(x_e) for sigmoid).
+ * Without offsets all tokens are one sequence.  Offsets ascend within [0, tokens]; sequence s is [offsets[s],
+ * offsets[s+1]); tokens of no sequence and tokens that are not valid are not looked at and have gradient 0; a sequence
+ * without valid tokens has loss 0.  A negative expert index is a dropped assignment: not counted.  An index >=
+ * experts makes its sequence's loss and gradient NaN, offsets that descend or leave the range make every loss NaN;
+ * nothing out of range is accessed.  Counts are whole-number atomics, sums of scores are fp32 in a fixed order. */
+typedef struct lpmm_b200_balance {
+  const void* logits;      /* row r begins at element (r / inner) * outer_stride + (r % inner) * inner_stride           */
+  void* grad;              /* [tokens, experts] contiguous, type of the logits (not for forward)                        */
+  const void* index;       /* [tokens, k] contiguous, index_bits wide                                                   */
+  const uint8_t* valid;    /* [tokens], 0 = not valid; or NULL                                                          */
+  const void* offsets;     /* [sequences + 1], offset_bits wide, or NULL (sequences = 1)                                */
+  const float* upstream;   /* backward only: [sequences]                                                                */
+  float* loss;             /* [sequences] (not for backward)                                                            */
+  int64_t* counts;         /* [sequences, experts]: written by forward, read by backward                                */
+  float* factor;           /* [sequences]: experts / (k n^2), written by forward, read by backward                      */
+  void* work;              /* lpmm_b200_balance_work_bytes, 16-byte aligned (not for backward)                          */
+  int64_t tokens, inner, outer_stride, inner_stride;
+  int64_t experts, k, sequences;
+  int32_t dtype, index_bits, offset_bits, score;
+  float grad_scale;
+  int32_t reserved;
+} lpmm_b200_balance;
+
+int64_t lpmm_b200_balance_work_bytes(int64_t tokens, int64_t experts, int64_t sequences);
+int lpmm_b200_balance_forward(const lpmm_b200_balance* b, void* stream);
+/* grad_scale * sum over sequences of upstream[s] * gradient of loss[s]. */
+int lpmm_b200_balance_backward(const lpmm_b200_balance* b, void* stream);
+/* Losses and counts, and grad_scale * the gradient of the losses' sum, in one call. */
+int lpmm_b200_balance_forward_backward(const lpmm_b200_balance* b, void* stream);
+
 /* Self-test hook (no counterpart in the reference; not part of any step).  The step kernels replace IEEE
  * division and square root and the reference's nearest-code search (fused_adamw_kernel.cu:27-49) by shorter
  * sequences that give the same result on a stated domain.  This runs one of those comparisons on the GPU over

@@ -58,14 +58,38 @@ class StepTensor(ctypes.Structure):
     ]
 
 
+class Distill(ctypes.Structure):
+    """``lpmm_b200_distill``"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "grad", "teacher", "index", "weights", "upstream", "loss", "work")]
+                + [(n, ctypes.c_int64) for n in ("rows", "inner", "outer_stride", "inner_stride", "vocab", "k")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "teacher_dtype", "index_bits", "reduction")]
+                + [("temperature", ctypes.c_float), ("grad_scale", ctypes.c_float)])
+
+
+class Balance(ctypes.Structure):
+    """``lpmm_b200_balance``"""
+    _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "grad", "index", "valid", "offsets", "upstream", "loss", "counts",
+                                                "factor", "work")]
+                + [(n, ctypes.c_int64) for n in ("tokens", "inner", "outer_stride", "inner_stride", "experts", "k",
+                                                 "sequences")]
+                + [(n, ctypes.c_int32) for n in ("dtype", "index_bits", "offset_bits", "score")]
+                + [("grad_scale", ctypes.c_float), ("reserved", ctypes.c_int32)])
+
+
 STATE_FP32, STATE_GROUP4, STATE_RANK1_4, STATE_FACTORED = 0, 1, 2, 3
 KIND_Q4 = 0
 KIND_FP32 = 1
+DTYPE_FP32 = 0
 DTYPE_BF16 = 1
 DTYPE_FP16 = 2
 FLAG_PARAMS_WITHIN_TOLERANCE = 1
 GROUP = 128
 PACK_GROUP = 2048
+REDUCE_NONE, REDUCE_SUM, REDUCE_MEAN = 0, 1, 2
+DISTILL_MAX_K = 1024
+DISTILL_MIN_T, DISTILL_MAX_T = 1.0 / 1024.0, 1024.0
+BALANCE_MAX_EXPERTS = 1024
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 STATIC_SCRATCH_BYTES = 8 * 1024 * 1024
 
 
@@ -139,6 +163,14 @@ def _load():
         "lpmm_b200_factored_scratch_bytes": (i64, [ctypes.POINTER(i64), i32]),
         "lpmm_b200_adamw4bit_factored_step_noalloc": (i32, [ctypes.POINTER(StepTensor), vp] + [d] * 6 + [vp]),
         "lpmm_b200_narrow_fp32": (i32, [vp, vp, i64, i32, vp]),
+        "lpmm_b200_distill_work_floats": (i64, [i64]),
+        "lpmm_b200_distill_forward": (i32, [ctypes.POINTER(Distill), vp]),
+        "lpmm_b200_distill_backward": (i32, [ctypes.POINTER(Distill), vp]),
+        "lpmm_b200_distill_forward_backward": (i32, [ctypes.POINTER(Distill), vp]),
+        "lpmm_b200_balance_work_bytes": (i64, [i64, i64, i64]),
+        "lpmm_b200_balance_forward": (i32, [ctypes.POINTER(Balance), vp]),
+        "lpmm_b200_balance_backward": (i32, [ctypes.POINTER(Balance), vp]),
+        "lpmm_b200_balance_forward_backward": (i32, [ctypes.POINTER(Balance), vp]),
         "lpmm_b200_test_exactness": (i32, [i32, vp, ctypes.c_uint64, i64, vp, vp]),
         "lpmm_b200_sgd4bit_step": (i32, [vp, vp, i64, vp, vp, i32, i32, vp, d, d, d, d, i32, i32, vp]),
     }

@@ -6,14 +6,19 @@ reference's signature and metadata dictionaries for the configurations of the lo
 -- ``scale_type`` 'group' (128 ... 4096) or 'rank1', ``quant_type`` 'nonlinear' or 'power-*',
 ``round_type`` 'real-nearest' or 'real-sr', 4 to 8 bits -- and run on the CUDA library; anything else
 raises.
+
+``topk_distillation`` and ``balance_loss`` (``losses.py``) are the losses next to the step: their
+gradients are what ``p.grad`` is made from.
 """
 import torch
 
 from . import _kernels
+from .losses import balance_loss, balance_loss_with_grad, topk_distillation, topk_distillation_with_grad
 
 __all__ = [
     "vectorwise_quant", "vectorwise_dequant", "create_general_qmap", "create_dynamic_map", "create_pow_map",
     "group_tensor", "recon_grouped_tensor", "get_sm3_statistics", "init_lpmm_generator",
+    "topk_distillation", "topk_distillation_with_grad", "balance_loss", "balance_loss_with_grad",
 ]
 
 lpmm_generator = None
