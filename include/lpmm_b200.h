@@ -485,7 +485,8 @@ int lpmm_b200_adamw4bit_factored_step_noalloc(const lpmm_b200_step_tensor* t, co
  * how the work is scheduled (no floating-point atomics). */
 typedef struct lpmm_b200_distill {
   const void* logits;      /* row r begins at element (r / inner) * outer_stride + (r % inner) * inner_stride           */
-  void* grad;              /* [rows, vocab] contiguous, type of the logits (not for forward)                            */
+  void* grad;              /* type of the logits, rows as theirs with the two strides below (not for forward); every    */
+                           /* row lies to the 16-byte boundaries as its row of logits does (BAD_SIZE otherwise)         */
   const void* teacher;     /* [rows, k] contiguous, teacher_dtype                                                       */
   const void* index;       /* [rows, k] contiguous, index_bits wide                                                     */
   const float* weights;    /* [rows], or NULL for 1                                                                     */
@@ -494,6 +495,7 @@ typedef struct lpmm_b200_distill {
   float* work;             /* lpmm_b200_distill_work_floats(rows) floats, 16-byte aligned; forward leaves in it what    */
                            /* backward reads                                                                            */
   int64_t rows, inner, outer_stride, inner_stride;
+  int64_t grad_outer_stride, grad_inner_stride;
   int64_t vocab;
   int64_t k;
   int32_t dtype, teacher_dtype, index_bits, reduction;

@@ -5,10 +5,13 @@
 //   loss = w T^2 sum_k p_k (log p_k - log q_{i_k})
 //   d loss / d x_v = w T (q_v - sum_{k: i_k = v} p_k)
 //
-// One CTA, or one cluster of CTAs that share the row's columns, takes a row: a pass with a running maximum and sum
-// gives the softmax statistics; the gradient is a second pass over the same columns, which the first one has left in
-// L2, then the K corrected entries are written over it.  All sums are fp32, the gradient is rounded once.
-// Bound by memory: a logit is read once and its gradient written once; an exponential per logit and pass.
+// A row takes two passes: a running maximum and sum give the softmax statistics, then q is written everywhere and the
+// K entries are written over it.  All sums are fp32, the gradient is rounded once.  Exponentials are 2^(x c - M) with
+// c = log2(e) / T and M = RN(m c), one fma and one hardware exponential each.
+// Three kernels, by the size of the problem (distill_launch):
+//   small   a row in the registers of one warp or of 128 threads
+//   stream  persistent CTAs, rows through a ring of shared memory filled by bulk copies
+//   split   a row's columns shared by a cluster of CTAs, for few rows
 #include <cooperative_groups.h>
 
 #include "loss_common.cuh"
@@ -20,10 +23,9 @@ namespace lpmm_b200 {
 enum { DISTILL_LOSS = 0, DISTILL_BOTH = 1, DISTILL_GRAD = 2 };
 
 constexpr int MAX_K = LPMM_B200_DISTILL_MAX_K;
-constexpr int HASH = 2 * MAX_K;  // at most half full
 
-// saved per row for the gradient: maximum and sum of the student's exponentials, the same of the teacher's.  The
-// teacher's sum is 0 for a row that has no part in the loss, NaN for one whose entries are invalid.
+// saved per row for the gradient: maximum and sum of the student's exponentials, the same of the teacher's (its sum is
+// NaN where an entry is invalid)
 struct __align__(16) RowStats {
   float m, s, tm, ts;
 };
@@ -38,16 +40,25 @@ struct DistillArgs {
   float* row_loss;
   RowStats* stats;
   const float* norm;  // 1 / sum of the weights, for the mean
-  long long rows, inner, outer_stride, inner_stride;
+  long long rows, inner, outer_stride, inner_stride, grad_outer_stride, grad_inner_stride;
   int vocab, k, teacher_dtype, index_bits, upstream_per_row;
   float temperature, c;  // c = log2(e) / T
   float scale;
-  int slice;  // columns per CTA of the cluster
+  int slice;             // split: columns per CTA of the cluster
+  int k_pad, hash_size;  // entries per row rounded up, slots of the table that finds an index given twice
+  int stages, resident;  // stream: chunks in the ring; a row stays in it for both passes
 };
 
 constexpr float LOWEST = -3.402823466e38f;
+constexpr float FAR = 1e38f;
+constexpr float LN2 = 0.6931471805599453f;
 
-// (m, s) stands for s * 2^(m c).  m starts at the lowest finite value: a -inf logit then adds 2^-inf = 0, and a NaN or
+// Where |m c| is beyond FAR (rows of the type's lowest value, above all) fp32 cannot hold M: such a row is done with
+// (x - m) c instead, which is exact there.
+__device__ __forceinline__ float ref_of(float m, float c) { return fmaxf(m * c, -FAR); }
+__device__ __forceinline__ bool far_off(float m, float c) { return !(fabsf(m * c) <= FAR); }
+
+// s stands for s * 2^ref_of(m).  m starts at the lowest finite value: a -inf logit then adds 2^-inf = 0, and a NaN or
 // +inf reaches s.
 struct Running {
   float m, s;
@@ -56,54 +67,88 @@ struct Running {
 __device__ __forceinline__ Running join(const Running& a, const Running& b, float c) {
   Running r;
   r.m = fmaxf(a.m, b.m);
-  r.s = a.s * ex2((a.m - r.m) * c) + b.s * ex2((b.m - r.m) * c);
+  const float ref = ref_of(r.m, c);
+  r.s = a.s * ex2(ref_of(a.m, c) - ref) + b.s * ex2(ref_of(b.m, c) - ref);
   return r;
 }
 
-template <int N>
-__device__ __forceinline__ void take(Running& a, const float* x, float c) {
-  float m = x[0];
+__device__ __forceinline__ Running warp_join(Running r, float c) {
+  float m = r.m;
 #pragma unroll
-  for (int i = 1; i < N; ++i) m = fmaxf(m, x[i]);
-  m = fmaxf(m, a.m);
-  float s = a.s * ex2((a.m - m) * c);
+  for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+  float s = r.s * ex2(ref_of(r.m, c) - ref_of(m, c));
 #pragma unroll
-  for (int i = 0; i < N; ++i) s += ex2((x[i] - m) * c);
-  a.m = m;
-  a.s = s;
+  for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+  return Running{m, s};
 }
 
-struct DistillSmem {
-  int idx[MAX_K];
-  float p[MAX_K];
-  float x[MAX_K];
-  int hash[HASH];
-  Running warp[32];
-  float red[32];
-  Running mine;  // this CTA's part of the row, read by the cluster
-  int bad, twice;
+// N vectors of 16 bytes
+template <typename T, int N>
+__device__ __forceinline__ void take(Running& r, const uint4* u, float c) {
+  using E = Elem<T>;
+  const float m = fmaxf(r.m, E::template maximum<N>(u));
+  const float ref = ref_of(m, c);
+  r.s *= ex2(ref_of(r.m, c) - ref);
+  r.m = m;
+  const f2 c2 = f2_splat(c), ref2 = f2_splat(-ref);
+  f2 sum = f2_splat(0.0f);
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    float x[E::VE];
+    E::unpack(u[j], x);
+#pragma unroll
+    for (int i = 0; i < E::VE; i += 2) {
+      float a, b;
+      f2_unpack(f2_fma(f2_pack(x[i], x[i + 1]), c2, ref2), a, b);
+      sum = f2_add(sum, f2_pack(ex2(a), ex2(b)));
+    }
+  }
+  float a, b;
+  f2_unpack(sum, a, b);
+  r.s += a + b;
+}
+
+__device__ __forceinline__ void take_one(Running& r, float x, float c) {
+  const float m = fmaxf(r.m, x), ref = ref_of(m, c);
+  r.s = r.s * ex2(ref_of(r.m, c) - ref) + ex2(fmaf(x, c, -ref));
+  r.m = m;
+}
+
+// The exponentials of one row: 2^(x c - M), or 2^((x - m) c) where M is out of range.
+struct Expo {
+  float m, c, ref;
+  bool far;
+  __device__ __forceinline__ Expo(float m_, float c_) : m(m_), c(c_), ref(ref_of(m_, c_)), far(far_off(m_, c_)) {}
+  __device__ __forceinline__ float log2_of(float x) const { return far ? (x - m) * c : fmaf(x, c, -ref); }
+  __device__ __forceinline__ float operator()(float x) const { return ex2(log2_of(x)); }
+  template <typename T>
+  __device__ __forceinline__ uint4 scaled(const uint4& u, float g) const {
+    using E = Elem<T>;
+    float x[E::VE];
+    E::unpack(u, x);
+    if (!far) {
+      const f2 c2 = f2_splat(c), ref2 = f2_splat(-ref), g2 = f2_splat(g);
+#pragma unroll
+      for (int i = 0; i < E::VE; i += 2) {
+        float a, b;
+        f2_unpack(f2_fma(f2_pack(x[i], x[i + 1]), c2, ref2), a, b);
+        f2_unpack(f2_mul(f2_pack(ex2(a), ex2(b)), g2), x[i], x[i + 1]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < E::VE; ++i) x[i] = g * ex2((x[i] - m) * c);
+    }
+    return E::pack(x);
+  }
 };
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = red[0];
-  for (int i = 1; i < (int)(blockDim.x >> 5); ++i) r = fmaxf(r, red[i]);
-  return r;
+template <typename T>
+__device__ __forceinline__ const T* logits_row(const DistillArgs& a, long long row) {
+  return reinterpret_cast<const T*>(a.logits) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.inner_stride;
 }
-
-__device__ __forceinline__ float block_sum(float v, float* red) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(~0u, v, o);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float r = red[0];
-  for (int i = 1; i < (int)(blockDim.x >> 5); ++i) r += red[i];
-  return r;
+template <typename T>
+__device__ __forceinline__ T* grad_row(const DistillArgs& a, long long row) {
+  return reinterpret_cast<T*>(a.grad) + (row / a.inner) * a.grad_outer_stride + (row % a.inner) * a.grad_inner_stride;
 }
 
 // Columns [lo, hi) of a row in steps of 16 bytes: up to VE - 1 single columns before the first boundary, vectors, the
@@ -111,7 +156,6 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
 struct Span {
   int lo, head, vecs, tail, tail_at;
 };
-
 template <typename T>
 __device__ __forceinline__ Span span_of(const T* row, int lo, int hi) {
   constexpr int VE = Elem<T>::VE;
@@ -125,193 +169,668 @@ __device__ __forceinline__ Span span_of(const T* row, int lo, int hi) {
   s.tail = hi - s.tail_at;
   return s;
 }
+// the single column of thread t, or -1 (threads 0 ... 2 VE - 3 have one)
+template <typename T>
+__device__ __forceinline__ int edge_of(const Span& s, int t) {
+  constexpr int VE = Elem<T>::VE;
+  if (t < VE - 1) return t < s.head ? s.lo + t : -1;
+  t -= VE - 1;
+  return t < s.tail ? s.tail_at + t : -1;
+}
+
+// ---------------------------------------------------------------------------------------------
+// A row's stored entries in shared memory, prepared by a team of threads (a warp, or a CTA)
+// ---------------------------------------------------------------------------------------------
+struct Warp {  // a team of 32 threads
+  static constexpr int SIZE = 32;
+  __device__ __forceinline__ int rank() const { return threadIdx.x & 31; }
+  __device__ __forceinline__ int size() const { return 32; }
+  __device__ __forceinline__ void sync() const { __syncwarp(); }
+  __device__ __forceinline__ bool any(bool v) const { return __any_sync(~0u, v); }
+  __device__ __forceinline__ float max(float v) const {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, d));
+    return v;
+  }
+  __device__ __forceinline__ float sum(float v) const {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+    return v;
+  }
+  __device__ __forceinline__ Running joined(Running r, float c) const { return warp_join(r, c); }
+};
+
+struct Block {  // all threads of the CTA (at most 16 warps)
+  float2* red;  // [2, 16] in shared memory
+  int turn = 0;
+  __device__ __forceinline__ explicit Block(float2* r) : red(r) {}
+  __device__ __forceinline__ int rank() const { return threadIdx.x; }
+  __device__ __forceinline__ int size() const { return blockDim.x; }
+  __device__ __forceinline__ void sync() const { __syncthreads(); }
+  __device__ __forceinline__ bool any(bool v) const { return __syncthreads_or(v); }
+  // two halves in turn: a barrier lies between a read and the next write of the same half
+  __device__ __forceinline__ float2* exchange(float2 v) {
+    float2* r = red + 16 * (turn ^= 1);
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    __syncthreads();
+    return r;
+  }
+  __device__ __forceinline__ float max(float v) {
+    const float2* r = exchange(make_float2(Warp().max(v), 0.0f));
+    v = r[0].x;
+    for (int i = 1; i < (int)(blockDim.x >> 5); ++i) v = fmaxf(v, r[i].x);
+    return v;
+  }
+  __device__ __forceinline__ float sum(float v) {
+    const float2* r = exchange(make_float2(Warp().sum(v), 0.0f));
+    v = r[0].x;
+    for (int i = 1; i < (int)(blockDim.x >> 5); ++i) v += r[i].x;
+    return v;
+  }
+  __device__ __forceinline__ Running joined(Running v, float c) {
+    v = warp_join(v, c);
+    const float2* r = exchange(make_float2(v.m, v.s));
+    const int n = blockDim.x >> 5, lane = threadIdx.x & 31;
+    v = lane < n ? Running{r[lane].x, r[lane].y} : Running{LOWEST, 0.0f};
+    return warp_join(v, c);
+  }
+};
+
+struct Entries {
+  int* idx;    // [k_pad], -1: no entry
+  float* p;    // [k_pad] t - tm, then the probability
+  float* x;    // [k_pad] the student's logit
+  int* hash;   // [hash_size], -1 when not in use
+  int* twice;  // an index occurs more than once
+};
+
+struct Teacher {
+  float w, tm, ts;
+  bool live;  // weight and entries: the row has a part in the loss
+};
+
+// Reads the row's entries.  GRAD: the statistics are in `st`.  The team's threads may read `e` afterwards.
+template <typename T, int MODE, typename Team>
+__device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, const T* x, Entries e, Team& team,
+                                           const RowStats& st) {
+  Teacher t;
+  t.w = a.weights ? a.weights[row] : 1.0f;
+  t.tm = LOWEST;
+  bool any = false, bad = false;
+  if (team.rank() == 0) *e.twice = 0;
+  for (int k = team.rank(); k < a.k; k += team.size()) {
+    const long long i = load_index(a.index, row * a.k + k, a.index_bits);
+    const float v = load_any(a.teacher, row * a.k + k, a.teacher_dtype);
+    const bool entry = i >= 0 && v != -__int_as_float(0x7f800000);
+    const bool in = entry && i < a.vocab;  // an index outside of the vocabulary is not followed
+    bad |= entry && !in;
+    any |= entry;
+    e.idx[k] = in ? (int)i : -1;
+    e.p[k] = v;
+    if (in && t.w != 0.0f) e.x[k] = Elem<T>::widen(x[i]);
+    if (entry) t.tm = fmaxf(t.tm, v);
+  }
+  t.live = team.any(any) && t.w != 0.0f;
+  t.ts = 0.0f;
+  if (!t.live) return t;
+  if (MODE == DISTILL_GRAD) {
+    t.tm = st.tm;
+    t.ts = st.ts;
+  } else {
+    t.tm = team.max(t.tm);
+    float sum = 0.0f;
+    for (int k = team.rank(); k < a.k; k += team.size())
+      if (e.idx[k] >= 0) sum += ex2((e.p[k] - t.tm) * a.c);
+    t.ts = team.sum(sum);
+    if (team.any(bad)) t.ts = nan_f();
+  }
+  for (int k = team.rank(); k < a.k; k += team.size()) {
+    const int i = e.idx[k];
+    e.p[k] = i >= 0 ? ex2((e.p[k] - t.tm) * a.c) / t.ts : 0.0f;
+    if (MODE != DISTILL_LOSS && i >= 0) {
+      for (unsigned h = ((unsigned)i * 2654435761u) >> 12;; ++h) {  // ends: the table is at most half full
+        const int was = atomicCAS(&e.hash[h & (a.hash_size - 1)], -1, i);
+        if (was == i) *e.twice = 1;
+        if (was == -1 || was == i) break;
+      }
+    }
+  }
+  team.sync();
+  if (MODE != DISTILL_LOSS)
+    for (int i = team.rank(); i < a.hash_size; i += team.size()) e.hash[i] = -1;
+  return t;
+}
+
+// sum_k p_k (log p_k - log q_k) of a prepared row, for all threads of the team.  log p_k from the probability itself
+// would lose the small ones: ln p = z ln2 with z = log2 p is read off p's own exponent argument, (t - tm) c - log2 ts.
+template <typename Team>
+__device__ __forceinline__ float divergence(const DistillArgs& a, long long row, const Teacher& t, Entries e, Team& team,
+                                            const Expo& ex, float s) {
+  float sum = 0.0f;
+  for (int k = team.rank(); k < a.k; k += team.size()) {
+    const float p = e.p[k];
+    if (e.idx[k] < 0 || p == 0.0f) continue;
+    const float z = (load_any(a.teacher, row * a.k + k, a.teacher_dtype) - t.tm) * a.c;
+    sum += p * (z - ex.log2_of(e.x[k]));
+  }
+  return LN2 * team.sum(sum) + (logf(s) - logf(t.ts));
+}
+
+// The entries' columns within [lo, hi): q - p, written over q.  After a barrier behind the stores of q.
+template <typename T, typename Team>
+__device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const Entries& e, const Team& team,
+                                              const Expo& ex, float gs, float G, int lo, int hi) {
+  const bool twice = *e.twice;
+  for (int k = team.rank(); k < a.k; k += team.size()) {
+    const int i = e.idx[k];
+    if (i < lo || i >= hi) continue;
+    float p = e.p[k];
+    if (twice) {  // an index that occurs several times: its first entry writes for all, in their order
+      bool first = true;
+      for (int j = 0; j < k; ++j) first &= e.idx[j] != i;
+      if (!first) continue;
+      for (int j = k + 1; j < a.k; ++j)
+        if (e.idx[j] == i) p += e.p[j];
+    }
+    g[i] = Elem<T>::narrow(gs * ex(e.x[k]) - G * p);
+  }
+}
+
+__device__ __forceinline__ float upstream_of(const DistillArgs& a, long long row) {
+  float up = a.scale * (a.norm ? *a.norm : 1.0f);
+  if (a.upstream) up *= a.upstream[a.upstream_per_row ? row : 0];
+  return up;
+}
+
+// Statistics of a row whose maximum lies beyond FAR, from its logits in memory.
+template <typename T, typename Team>
+__device__ __noinline__ float far_sum(const DistillArgs& a, const T* x, int lo, int hi, float m, Team& team) {
+  float s = 0.0f;
+  for (int v = lo + team.rank(); v < hi; v += team.size()) s += ex2((Elem<T>::widen(x[v]) - m) * a.c);
+  return team.sum(s);
+}
+
+// ---------------------------------------------------------------------------------------------
+// small: a row in the registers of GT threads, all of its loads in flight at once
+// ---------------------------------------------------------------------------------------------
+constexpr int SMALL_VECS = 8;
+
+__host__ __device__ constexpr size_t entry_bytes(int k_pad, int hash_size) { return 12 * (size_t)k_pad + 4 * (size_t)hash_size; }
+
+__device__ __forceinline__ Entries entries_at(char* p, const DistillArgs& a, int* twice) {
+  Entries e;
+  e.idx = reinterpret_cast<int*>(p);
+  e.p = reinterpret_cast<float*>(p + 4 * a.k_pad);
+  e.x = reinterpret_cast<float*>(p + 8 * a.k_pad);
+  e.hash = reinterpret_cast<int*>(p + 12 * a.k_pad);
+  e.twice = twice;
+  return e;
+}
+
+template <typename T, int MODE, typename Team>
+__device__ __forceinline__ void small_row(const DistillArgs& a, long long row, Entries e, Team& team) {
+  using E = Elem<T>;
+  const T* x = logits_row<T>(a, row);
+  const Span o = span_of(x, 0, a.vocab);
+  const int t = team.rank();
+  const bool skip = a.weights && a.weights[row] == 0.0f;
+  uint4 u[SMALL_VECS];
+  const uint4* xv = reinterpret_cast<const uint4*>(x + o.head);
+#pragma unroll
+  for (int j = 0; j < SMALL_VECS; ++j) {
+    const int i = t + j * team.size();
+    u[j] = i < o.vecs && !skip ? xv[i] : E::none();
+  }
+  const int at = edge_of<T>(o, t);
+  const float edge = at >= 0 && !skip ? E::widen(x[at]) : -__int_as_float(0x7f800000);
+  RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+  if (MODE == DISTILL_GRAD) st = a.stats[row];
+  const Teacher tch = prepare<T, MODE>(a, row, x, e, team, st);
+  if (MODE != DISTILL_GRAD) {
+    Running r{LOWEST, 0.0f};
+    take<T, SMALL_VECS>(r, u, a.c);
+    take_one(r, edge, a.c);
+    r = team.joined(r, a.c);
+    st.m = r.m;
+    st.s = r.s;
+    if (tch.live && far_off(r.m, a.c)) {
+      st.s = far_sum(a, x, 0, a.vocab, r.m, team);
+      if (st.s == 0.0f) st.s = nan_f();  // every logit -inf: no distribution
+    }
+  }
+  const Expo ex(st.m, a.c);
+  if (MODE != DISTILL_GRAD) {
+    const float d = tch.live ? divergence(a, row, tch, e, team, ex, st.s) : 0.0f;
+    if (t == 0) {
+      a.row_loss[row] = tch.live ? tch.w * a.temperature * a.temperature * d : 0.0f;
+      a.stats[row] = RowStats{st.m, st.s, tch.tm, tch.ts};
+    }
+  }
+  if (MODE == DISTILL_LOSS) return;
+  T* g = grad_row<T>(a, row);
+  uint4* gv = reinterpret_cast<uint4*>(g + o.head);
+  const float G = tch.live ? upstream_of(a, row) * tch.w * a.temperature + (tch.ts - tch.ts) : 0.0f;
+  const float gs = tch.live ? G / st.s : 0.0f;
+#pragma unroll
+  for (int j = 0; j < SMALL_VECS; ++j) {
+    const int i = t + j * team.size();
+    if (i < o.vecs) gv[i] = tch.live ? ex.scaled<T>(u[j], gs) : make_uint4(0, 0, 0, 0);
+  }
+  if (at >= 0) g[at] = E::narrow(tch.live ? gs * ex(edge) : 0.0f);
+  team.sync();
+  if (tch.live) write_entries(a, g, e, team, ex, gs, G, 0, a.vocab);
+}
+
+template <typename T, int MODE, int GT>
+__global__ void __launch_bounds__(128) distill_small_kernel(const DistillArgs a) {
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float2 red[32];
+  __shared__ int twice[128 / GT];
+  const int mine = threadIdx.x / GT;
+  const long long row = (long long)blockIdx.x * (128 / GT) + mine;
+  const Entries e = entries_at(smem + mine * entry_bytes(a.k_pad, a.hash_size), a, &twice[mine]);
+  if (MODE != DISTILL_LOSS) {
+    for (int i = threadIdx.x % GT; i < a.hash_size; i += GT) e.hash[i] = -1;
+  }
+  pdl_wait();
+  if (GT == 32) {
+    __syncwarp();
+    if (row >= a.rows) return;
+    Warp team;
+    small_row<T, MODE>(a, row, e, team);
+  } else {
+    __syncthreads();
+    Block team(red);
+    small_row<T, MODE>(a, row, e, team);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// stream: persistent CTAs; one warp copies the rows into a ring of chunks, one prepares the entries of the next row,
+// eight take the passes
+// ---------------------------------------------------------------------------------------------
+constexpr int CHUNK = 8192;
+constexpr int CWARPS = 8, CTHREADS = CWARPS * 32;
+constexpr int PER = CHUNK / 16 / CTHREADS;  // vectors per thread and chunk
+constexpr int MAX_STAGES = 28;
+
+struct StreamRow {  // what the consumers are told about a row, and what they tell
+  Teacher t;
+  int skip, twice;
+  float m, s, G;
+};
+
+struct StreamSmem {
+  unsigned long long full[MAX_STAGES], empty[MAX_STAGES];
+  unsigned long long told[2], freed[2], stat[2];  // entries ready / no longer read / statistics of the row known
+  StreamRow row[2];
+  float2 red[2][CWARPS];
+  int failed;
+};
+
+// the consumers as a team: named barrier 1
+struct Consumers {
+  float2 (*red)[CWARPS];
+  int turn = 0;
+  __device__ __forceinline__ explicit Consumers(float2 (*r)[CWARPS]) : red(r) {}
+  __device__ __forceinline__ int rank() const { return threadIdx.x; }
+  __device__ __forceinline__ int size() const { return CTHREADS; }
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync 1, %0;" ::"n"(CTHREADS) : "memory"); }
+  __device__ __forceinline__ float2* exchange(float2 v) {
+    float2* r = red[turn ^= 1];
+    if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
+    sync();
+    return r;
+  }
+  __device__ __forceinline__ float sum(float v) {
+    const float2* r = exchange(make_float2(Warp().sum(v), 0.0f));
+    v = r[0].x;
+    for (int i = 1; i < CWARPS; ++i) v += r[i].x;
+    return v;
+  }
+  __device__ __forceinline__ Running joined(Running v, float c) {
+    v = warp_join(v, c);
+    const float2 o = exchange(make_float2(v.m, v.s))[threadIdx.x % CWARPS];
+    float m = o.x;
+#pragma unroll
+    for (int d = CWARPS / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    float s = o.y * ex2(ref_of(o.x, c) - ref_of(m, c));
+#pragma unroll
+    for (int d = CWARPS / 2; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+    return Running{m, s};
+  }
+};
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(512) distill_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(CTHREADS + 64, 2) distill_stream_kernel(const DistillArgs a) {
   using E = Elem<T>;
-  constexpr int VE = E::VE;
-  __shared__ DistillSmem sm;
+  extern __shared__ __align__(16) char smem[];
+  char* ring = smem;
+  StreamSmem& sm = *reinterpret_cast<StreamSmem*>(smem + (size_t)a.stages * CHUNK);
+  char* entry_mem = smem + (size_t)a.stages * CHUNK + (sizeof(StreamSmem) + 15) / 16 * 16;
+  const size_t per_slot = 12 * (size_t)a.k_pad;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(&sm.full[i], 1);
+      mbar_init(&sm.empty[i], CWARPS);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&sm.told[i], 1);
+      mbar_init(&sm.freed[i], CWARPS);
+      mbar_init(&sm.stat[i], 1);
+    }
+    sm.failed = 0;
+    mbar_fence();
+  }
+  int* hash = reinterpret_cast<int*>(entry_mem + 2 * per_slot);
+  for (int i = threadIdx.x; i < a.hash_size; i += blockDim.x) hash[i] = -1;
+  __syncthreads();
+  const long long grid = gridDim.x;
+  // passes over the chunks: once where the row stays in the ring, or only one pass is made
+  const int loads = MODE == DISTILL_BOTH && !a.resident ? 2 : 1;
+
+  if (warp == CWARPS) {  // the copies
+    int st = 0, fills = 0;
+    uint32_t phase = 0, skips = 0;
+    long long it = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += grid, ++it) {
+      if ((it & 31) == 0) {
+        const long long r = row + lane * grid;
+        skips = __ballot_sync(~0u, a.weights && r < a.rows && a.weights[r] == 0.0f);
+      }
+      if (skips >> (it & 31) & 1) continue;
+      if (lane == 0) {
+        const T* x = logits_row<T>(a, row);
+        const Span o = span_of(x, 0, a.vocab);
+        const char* from = reinterpret_cast<const char*>(x + o.head);
+        const long long bytes = (long long)o.vecs * 16;
+        for (int pass = 0; pass < loads; ++pass)
+          for (long long at = 0; at < bytes; at += CHUNK) {
+            if (fills >= a.stages) mbar_wait(&sm.empty[st], phase ^ 1, &sm.failed);
+            if (*(volatile int*)&sm.failed) break;  // nothing is copied any more
+            const uint32_t n = (uint32_t)min((long long)CHUNK, bytes - at);
+            mbar_expect(&sm.full[st], n);
+            bulk_load(ring + (size_t)st * CHUNK, from + at, n, &sm.full[st]);
+            if (fills < a.stages) ++fills;
+            if (++st == a.stages) st = 0, phase ^= 1;
+          }
+      }
+      __syncwarp();
+    }
+    if (lane == 0 && *(volatile int*)&sm.failed) {  // a wait ran out: the copies under way still have to land
+      for (int i = 0; i < fills; ++i) {
+        if (--st < 0) st = a.stages - 1, phase ^= 1;
+        mbar_wait_landed(&sm.full[st], phase);
+      }
+    }
+  } else if (warp == CWARPS + 1) {  // the entries
+    pdl_wait();  // *norm
+    Warp team;
+    long long it = 0;
+    long long before = -1;  // the row whose loss is still to be written
+    for (long long row = blockIdx.x;; row += grid, ++it) {
+      const int slot = it & 1;
+      if (row < a.rows) {
+        if (it >= 2) mbar_wait(&sm.freed[slot], ((it >> 1) - 1) & 1, &sm.failed);
+        StreamRow& h = sm.row[slot];
+        Entries e;
+        e.idx = reinterpret_cast<int*>(entry_mem + slot * per_slot);
+        e.p = reinterpret_cast<float*>(e.idx + a.k_pad);
+        e.x = e.p + a.k_pad;
+        e.hash = hash;
+        e.twice = &h.twice;
+        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+        if (MODE == DISTILL_GRAD) st = a.stats[row];
+        const Teacher t = prepare<T, MODE>(a, row, logits_row<T>(a, row), e, team, st);
+        if (lane == 0) {
+          h.t = t;
+          h.skip = t.w == 0.0f;
+          if (MODE == DISTILL_GRAD) h.m = st.m, h.s = st.s;
+          if (MODE != DISTILL_LOSS) h.G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);
+          mbar_arrive(&sm.told[slot]);
+        }
+        __syncwarp();
+      }
+      if (MODE != DISTILL_GRAD && before >= 0) {  // the loss of the row before
+        const int was = slot ^ 1;
+        mbar_wait(&sm.stat[was], ((it - 1) >> 1) & 1, &sm.failed);
+        StreamRow& h = sm.row[was];
+        const Teacher t = h.t;
+        Entries e;
+        e.idx = reinterpret_cast<int*>(entry_mem + was * per_slot);
+        e.p = reinterpret_cast<float*>(e.idx + a.k_pad);
+        e.x = e.p + a.k_pad;
+        float loss = 0.0f;
+        if (t.live) {
+          const Expo ex(h.m, a.c);
+          loss = t.w * a.temperature * a.temperature * divergence(a, before, t, e, team, ex, h.s);
+        }
+        if (lane == 0) {
+          a.row_loss[before] = loss;
+          a.stats[before] = RowStats{h.m, h.s, t.tm, t.ts};
+        }
+        __syncwarp();
+      }
+      if (row >= a.rows) break;
+      before = row;
+    }
+  } else {
+    const int tid = threadIdx.x;
+    Consumers team(sm.red);
+    int st = 0;
+    uint32_t phase = 0;
+    long long it = 0;
+    for (long long row = blockIdx.x; row < a.rows; row += grid, ++it) {
+      const int slot = it & 1;
+      const T* x = logits_row<T>(a, row);
+      T* g = MODE == DISTILL_LOSS ? nullptr : grad_row<T>(a, row);
+      const Span o = span_of(x, 0, a.vocab);
+      const int chunks = (int)(((long long)o.vecs * 16 + CHUNK - 1) / CHUNK);
+      const int at = edge_of<T>(o, tid);
+      float edge = at >= 0 ? E::widen(x[at]) : -__int_as_float(0x7f800000);
+      uint4* gv = MODE == DISTILL_LOSS ? nullptr : reinterpret_cast<uint4*>(g + o.head);
+      mbar_wait(&sm.told[slot], (it >> 1) & 1, &sm.failed);
+      StreamRow& h = sm.row[slot];
+      const Teacher t = h.t;
+      const int skip = h.skip;
+      if (!t.live) {
+        if (!skip)  // weight, but no entry: the copies are under way
+          for (int i = 0; i < chunks * loads; ++i) {
+            mbar_wait(&sm.full[st], phase, &sm.failed);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.empty[st]);
+            if (++st == a.stages) st = 0, phase ^= 1;
+          }
+        if (MODE != DISTILL_LOSS) {
+          for (int i = tid; i < o.vecs; i += CTHREADS) gv[i] = make_uint4(0, 0, 0, 0);
+          if (at >= 0) g[at] = E::narrow(0.0f);
+        }
+        if (MODE != DISTILL_GRAD && tid == 0) {
+          h.m = 0.0f, h.s = 1.0f;
+          mbar_arrive(&sm.stat[slot]);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.freed[slot]);
+        continue;
+      }
+      float m, s;
+      const int st0 = st;
+      if (MODE == DISTILL_GRAD) {
+        m = h.m, s = h.s;
+      } else {
+        Running r{LOWEST, 0.0f};
+        for (int i = 0; i < chunks; ++i) {
+          mbar_wait(&sm.full[st], phase, &sm.failed);
+          const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)st * CHUNK);
+          const int n = o.vecs - i * (CHUNK / 16);
+          uint4 u[PER];
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const int v = tid + j * CTHREADS;
+            u[j] = v < n ? buf[v] : E::none();
+          }
+          if (MODE == DISTILL_LOSS || !a.resident) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sm.empty[st]);
+          }
+          take<T, PER>(r, u, a.c);
+          if (++st == a.stages) st = 0, phase ^= 1;
+        }
+        take_one(r, edge, a.c);
+        r = team.joined(r, a.c);
+        m = r.m, s = r.s;
+        if (far_off(m, a.c)) {
+          s = far_sum(a, x, 0, a.vocab, m, team);
+          if (s == 0.0f) s = nan_f();  // every logit -inf: no distribution
+        }
+        if (tid == 0) {
+          h.m = m, h.s = s;
+          mbar_arrive(&sm.stat[slot]);
+        }
+        __syncwarp();
+      }
+      if (MODE != DISTILL_LOSS) {
+        const Expo ex(m, a.c);
+        const float G = h.G, gs = G / s;
+        int s2 = MODE == DISTILL_BOTH && a.resident ? st0 : st;
+        for (int i = 0; i < chunks; ++i) {
+          if (MODE == DISTILL_GRAD || !a.resident) {
+            mbar_wait(&sm.full[s2], phase, &sm.failed);
+          }
+          const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)s2 * CHUNK);
+          const int first = i * (CHUNK / 16), n = o.vecs - first;
+          uint4 u[PER];
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const int v = tid + j * CTHREADS;
+            if (v < n) u[j] = buf[v];
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&sm.empty[s2]);
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            const int v = tid + j * CTHREADS;
+            if (v < n) gv[first + v] = ex.scaled<T>(u[j], gs);
+          }
+          if (++s2 == a.stages) {
+            s2 = 0;
+            if (MODE == DISTILL_GRAD || !a.resident) phase ^= 1;
+          }
+        }
+        if (MODE == DISTILL_GRAD || !a.resident) st = s2;
+        if (at >= 0) g[at] = E::narrow(gs * ex(edge));
+        team.sync();
+        Entries e;
+        e.idx = reinterpret_cast<int*>(entry_mem + slot * per_slot);
+        e.p = reinterpret_cast<float*>(e.idx + a.k_pad);
+        e.x = e.p + a.k_pad;
+        e.hash = nullptr;
+        e.twice = &h.twice;
+        write_entries(a, g, e, team, ex, gs, G, 0, a.vocab);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.freed[slot]);
+    }
+  }
+  __syncthreads();
+  if (sm.failed)  // a wait ran out (it never has): what this CTA wrote is not to be taken for a result
+    for (long long row = blockIdx.x + threadIdx.x * grid; row < a.rows; row += blockDim.x * grid) {
+      if (MODE != DISTILL_GRAD) a.row_loss[row] = nan_f();
+      if (MODE != DISTILL_LOSS) grad_row<T>(a, row)[0] = E::narrow(nan_f());
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// split: one CTA, or one cluster of CTAs that share the columns, per row
+// ---------------------------------------------------------------------------------------------
+template <typename T, int MODE>
+__global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a) {
+  using E = Elem<T>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ float2 red[32];
+  __shared__ int twice;
+  __shared__ Running mine;  // this CTA's part of the row, read by the cluster
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const long long row = blockIdx.x / parts;
   const int tid = threadIdx.x, nthr = blockDim.x;
   const int lo = min(part * a.slice, a.vocab), hi = min(lo + a.slice, a.vocab);
-  const T* x = reinterpret_cast<const T*>(a.logits) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.inner_stride;
-  T* g = MODE == DISTILL_LOSS ? nullptr : reinterpret_cast<T*>(a.grad) + row * a.vocab;
-  const float w = a.weights ? a.weights[row] : 1.0f;
-
-  // the teacher's entries; an index outside the vocabulary makes the row NaN and is not followed
-  if (tid == 0) sm.bad = sm.twice = 0;
+  const T* x = logits_row<T>(a, row);
+  T* g = MODE == DISTILL_LOSS ? nullptr : grad_row<T>(a, row);
+  Entries e = entries_at(smem, a, &twice);
+  Block team(red);
   if (MODE != DISTILL_LOSS)
-    for (int i = tid; i < HASH; i += nthr) sm.hash[i] = -1;
+    for (int i = tid; i < a.hash_size; i += nthr) e.hash[i] = -1;
   __syncthreads();
-  float tm = LOWEST;
-  bool any = false;
-  for (int k = tid; k < a.k; k += nthr) {
-    const long long i = load_index(a.index, row * a.k + k, a.index_bits);
-    const float t = load_any(a.teacher, row * a.k + k, a.teacher_dtype);
-    const bool entry = i >= 0 && t != -__int_as_float(0x7f800000);
-    if (entry && i >= a.vocab) sm.bad = 1;
-    sm.idx[k] = entry && i < a.vocab ? (int)i : -1;
-    sm.p[k] = t;
-    if (entry) {
-      any = true;
-      tm = fmaxf(tm, t);
-    }
-  }
-  const bool live = __syncthreads_or(any) && w != 0.0f;
-  const bool bad = sm.bad;
-  if (!live) {  // uniform over the cluster: every CTA of it has read the same entries
+  pdl_wait();
+  RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+  if (MODE == DISTILL_GRAD) st = a.stats[row];
+  const Teacher t = prepare<T, MODE>(a, row, x, e, team, st);
+  if (!t.live) {  // uniform over the cluster: every CTA of it has read the same entries
     if (MODE != DISTILL_LOSS) {
       const Span o = span_of(g, lo, hi);
-      if (tid < o.head) g[o.lo + tid] = E::narrow(0.0f);
+      const int at = edge_of<T>(o, tid);
       uint4* gv = reinterpret_cast<uint4*>(g + o.lo + o.head);
       for (int i = tid; i < o.vecs; i += nthr) gv[i] = make_uint4(0, 0, 0, 0);
-      if (tid < o.tail) g[o.tail_at + tid] = E::narrow(0.0f);
+      if (at >= 0) g[at] = E::narrow(0.0f);
     }
     if (MODE != DISTILL_GRAD && tid == 0 && part == 0) {
       a.row_loss[row] = 0.0f;
-      a.stats[row] = RowStats{0.0f, 1.0f, 0.0f, 0.0f};
+      a.stats[row] = st;
     }
     return;
   }
-  float ts, m, s;
-  if (MODE == DISTILL_GRAD) {
-    const RowStats st = a.stats[row];
-    tm = st.tm, ts = st.ts, m = st.m, s = st.s;
-    for (int k = tid; k < a.k; k += nthr) sm.p[k] = sm.idx[k] >= 0 ? ex2((sm.p[k] - tm) * a.c) / ts : 0.0f;
-  } else {
-    tm = block_max(tm, sm.red);
-    float sum = 0.0f;
-    for (int k = tid; k < a.k; k += nthr)
-      if (sm.idx[k] >= 0) sum += ex2((sm.p[k] - tm) * a.c);
-    ts = block_sum(sum, sm.red);
-    if (bad) ts = nan_f();
-
+  if (MODE != DISTILL_GRAD) {
     // one pass over the row: running maximum and sum
     const Span o = span_of(x, lo, hi);
+    const int at = edge_of<T>(o, tid);
+    const float edge = at >= 0 ? E::widen(x[at]) : -__int_as_float(0x7f800000);
     Running r{LOWEST, 0.0f};
-    if (tid < o.head) {
-      const float v = E::widen(x[o.lo + tid]);
-      take<1>(r, &v, a.c);
-    }
-    if (tid < o.tail) {
-      const float v = E::widen(x[o.tail_at + tid]);
-      take<1>(r, &v, a.c);
-    }
     const uint4* xv = reinterpret_cast<const uint4*>(x + o.lo + o.head);
-    int i = tid;
-    for (; i + 3 * nthr < o.vecs; i += 4 * nthr) {
-      float v[4 * VE];
+    for (int i = tid; i < o.vecs; i += 4 * nthr) {
       uint4 u[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = xv[i + j * nthr];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) E::unpack(u[j], v + j * VE);
-      take<4 * VE>(r, v, a.c);
+      for (int j = 0; j < 4; ++j) u[j] = i + j * nthr < o.vecs ? xv[i + j * nthr] : E::none();
+      take<T, 4>(r, u, a.c);
     }
-    for (; i < o.vecs; i += nthr) {
-      float v[VE];
-      E::unpack(xv[i], v);
-      take<VE>(r, v, a.c);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-      Running b;
-      b.m = __shfl_xor_sync(~0u, r.m, d);
-      b.s = __shfl_xor_sync(~0u, r.s, d);
-      r = join(r, b, a.c);
-    }
-    if ((tid & 31) == 0) sm.warp[tid >> 5] = r;
-    __syncthreads();
-    r = sm.warp[0];
-    for (int j = 1; j < (nthr >> 5); ++j) r = join(r, sm.warp[j], a.c);
+    take_one(r, edge, a.c);
+    r = team.joined(r, a.c);
     if (parts > 1) {
-      if (tid == 0) sm.mine = r;
+      if (tid == 0) mine = r;
       cluster.sync();
-      r = *cluster.map_shared_rank(&sm.mine, 0);
-      for (int j = 1; j < parts; ++j) r = join(r, *cluster.map_shared_rank(&sm.mine, j), a.c);
+      r = *cluster.map_shared_rank(&mine, 0);
+      for (int j = 1; j < parts; ++j) r = join(r, *cluster.map_shared_rank(&mine, j), a.c);
       cluster.sync();  // nobody leaves while its part is still read
     }
-    m = r.m;
-    s = r.s == 0.0f ? nan_f() : r.s;  // every logit -inf: no distribution
-
-    if (part == 0) {
-      const float inv_t = 1.0f / a.temperature, log_ts = logf(ts);
-      float sum_l = 0.0f;
-      for (int k = tid; k < a.k; k += nthr) {
-        if (sm.idx[k] < 0) continue;
-        const float z = sm.p[k] - tm, p = ex2(z * a.c) / ts;
-        if (p != 0.0f) sum_l += p * ((z - (E::widen(x[sm.idx[k]]) - m)) * inv_t - log_ts);
-      }
-      sum_l = block_sum(sum_l, sm.red);
-      if (tid == 0) {
-        a.row_loss[row] = w * a.temperature * a.temperature * (sum_l + logf(s)) + (ts - ts);
-        a.stats[row] = RowStats{m, s, tm, ts};
-      }
-    }
-    if (MODE == DISTILL_LOSS) return;
-    __syncthreads();
-    for (int k = tid; k < a.k; k += nthr) sm.p[k] = sm.idx[k] >= 0 ? ex2((sm.p[k] - tm) * a.c) / ts : 0.0f;
-  }
-
-  // the gradient: q everywhere, then the entries of this part of the row
-  float up = a.scale * (a.norm ? *a.norm : 1.0f);
-  if (a.upstream) up *= a.upstream[a.upstream_per_row ? row : 0];
-  const float G = up * w * a.temperature + (ts - ts);  // NaN for a row with invalid entries
-  const float gs = G / s;
-  for (int k = tid; k < a.k; k += nthr) {
-    const int i = sm.idx[k];
-    if (i < lo || i >= hi) continue;
-    sm.x[k] = E::widen(x[i]);
-    for (unsigned h = (unsigned)i * 2654435761u >> 16;; ++h) {  // ends: the table is at most half full
-      const int was = atomicCAS(&sm.hash[h % HASH], -1, i);
-      if (was == -1) break;
-      if (was == i) {
-        sm.twice = 1;
-        break;
-      }
+    st.m = r.m;
+    st.s = r.s;
+    if (far_off(r.m, a.c)) {  // every CTA over the whole row: rare, and needs no exchange
+      st.s = far_sum(a, x, 0, a.vocab, r.m, team);
+      if (st.s == 0.0f) st.s = nan_f();  // every logit -inf: no distribution
     }
   }
+  const Expo ex(st.m, a.c);
+  if (MODE != DISTILL_GRAD && part == 0) {
+    const float d = divergence(a, row, t, e, team, ex, st.s);
+    if (tid == 0) {
+      a.row_loss[row] = t.w * a.temperature * a.temperature * d;
+      a.stats[row] = RowStats{st.m, st.s, t.tm, t.ts};
+    }
+  }
+  if (MODE == DISTILL_LOSS) return;
+  const float G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);  // NaN for a row with invalid entries
+  const float gs = G / st.s;
   {
     const Span o = span_of(g, lo, hi);
-    if (tid < o.head) g[o.lo + tid] = E::narrow(gs * ex2((E::widen(x[o.lo + tid]) - m) * a.c));
-    if (tid < o.tail) g[o.tail_at + tid] = E::narrow(gs * ex2((E::widen(x[o.tail_at + tid]) - m) * a.c));
+    const int at = edge_of<T>(o, tid);
+    if (at >= 0) g[at] = E::narrow(gs * ex(E::widen(x[at])));
     uint4* gv = reinterpret_cast<uint4*>(g + o.lo + o.head);
-    const T* xs = x + o.lo + o.head;
-    if (((uintptr_t)xs & 15) == 0) {
-      const uint4* xv = reinterpret_cast<const uint4*>(xs);
-      for (int i = tid; i < o.vecs; i += nthr) {
-        float v[VE];
-        E::unpack(xv[i], v);
-#pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = gs * ex2((v[j] - m) * a.c);
-        gv[i] = E::pack(v);
-      }
-    } else {  // rows of logits and gradient that lie differently to the 16-byte boundaries: single loads
-      for (int i = tid; i < o.vecs; i += nthr) {
-        float v[VE];
-#pragma unroll
-        for (int j = 0; j < VE; ++j) v[j] = gs * ex2((E::widen(xs[i * VE + j]) - m) * a.c);
-        gv[i] = E::pack(v);
-      }
-    }
+    const uint4* xv = reinterpret_cast<const uint4*>(x + o.lo + o.head);
+    for (int i = tid; i < o.vecs; i += nthr) gv[i] = ex.scaled<T>(xv[i], gs);
   }
   __syncthreads();
-  const bool twice = sm.twice;
-  for (int k = tid; k < a.k; k += nthr) {
-    const int i = sm.idx[k];
-    if (i < lo || i >= hi) continue;
-    float p = sm.p[k];
-    if (twice) {  // an index that occurs several times: its first entry writes for all, in their order
-      bool first = true;
-      for (int j = 0; j < k; ++j) first &= sm.idx[j] != i;
-      if (!first) continue;
-      for (int j = k + 1; j < a.k; ++j)
-        if (sm.idx[j] == i) p += sm.p[j];
-    }
-    g[i] = E::narrow(gs * ex2((sm.x[k] - m) * a.c) - G * p);
-  }
+  write_entries(a, g, e, team, ex, gs, G, lo, hi);
 }
 
 // One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double.
@@ -319,6 +838,8 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
                                                               const float* __restrict__ weights, long long rows, int mean,
                                                               float* __restrict__ loss, float* __restrict__ norm) {
   __shared__ double red[2][32];
+  pdl_start_next();
+  pdl_wait();
   double l = 0.0, w = 0.0;
   for (long long i = threadIdx.x; i < rows; i += blockDim.x) {
     if (row_loss) l += row_loss[i];
@@ -354,29 +875,72 @@ static int distill_check(const lpmm_b200_distill* d, int mode) {
   if (mode != DISTILL_GRAD && !d->loss && (d->rows || d->reduction != LPMM_B200_REDUCE_NONE)) return LPMM_B200_ERR_NULL_POINTER;
   if (mode == DISTILL_GRAD && !d->upstream) return LPMM_B200_ERR_NULL_POINTER;
   if ((uintptr_t)d->work & 15) return LPMM_B200_ERR_BAD_SIZE;
+  if (d->rows && mode != DISTILL_LOSS) {  // 16-byte accesses follow both
+    const int64_t size = d->dtype == LPMM_B200_DTYPE_FP32 ? 4 : 2;
+    if ((((uintptr_t)d->logits - (uintptr_t)d->grad) & 15) || (d->outer_stride - d->grad_outer_stride) * size % 16 ||
+        (d->inner_stride - d->grad_inner_stride) * size % 16)
+      return LPMM_B200_ERR_BAD_SIZE;
+  }
   return LPMM_B200_OK;
 }
 
+template <typename K>
+static cudaError_t launch(K kernel, const DistillArgs& a, long long grid, int threads, size_t smem, int cluster, bool after,
+                          cudaStream_t stream) {
+  if (smem > 40 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  if (after) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+// `after`: the kernel before it in the stream is this call's sum of the weights
 template <typename T, int MODE>
-static cudaError_t distill_launch(DistillArgs& a, cudaStream_t stream) {
+static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t stream) {
+  constexpr int VE = Elem<T>::VE;
+  const long long row_bytes = (long long)a.vocab * sizeof(T);
+  const size_t entries = entry_bytes(a.k_pad, a.hash_size);
+  if (row_bytes <= 16 * SMALL_VECS * 32 && a.k <= 256)
+    return launch(distill_small_kernel<T, MODE, 32>, a, (a.rows + 3) / 4, 128, 4 * entries, 1, after, stream);
+  if (row_bytes <= 16 * SMALL_VECS * 128)
+    return launch(distill_small_kernel<T, MODE, 128>, a, a.rows, 128, entries, 1, after, stream);
+  const int sms = num_sms();
+  if (a.rows >= sms) {
+    constexpr size_t LIMIT = 113 * 1024;  // two CTAs per SM
+    const size_t rest = (sizeof(StreamSmem) + 15) / 16 * 16 + entries + 12 * (size_t)a.k_pad;
+    a.stages = (int)((LIMIT - rest) / CHUNK);
+    if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
+    const long long chunks = (row_bytes + CHUNK - 1) / CHUNK;
+    a.resident = MODE == DISTILL_BOTH && chunks <= a.stages * 3 / 4;
+    const long long grid = a.rows < 2 * sms ? a.rows : 2 * sms;
+    return launch(distill_stream_kernel<T, MODE>, a, grid, CTHREADS + 64, a.stages * CHUNK + rest, 1, after, stream);
+  }
   // few rows: their columns are shared by clusters of up to 8 CTAs, so that all SMs have work
   int parts = 1;
-  const int vecs = (a.vocab + Elem<T>::VE - 1) / Elem<T>::VE;
-  while (parts < 8 && a.rows * parts < 2ll * num_sms() && vecs / (parts * 2) >= 512) parts *= 2;
-  a.slice = ((vecs + parts - 1) / parts + 7) / 8 * 8 * Elem<T>::VE;
-  const int per = a.slice / Elem<T>::VE;
+  const int vecs = (a.vocab + VE - 1) / VE;
+  while (parts < 8 && a.rows * parts < 2ll * sms && vecs / (parts * 2) >= 512) parts *= 2;
+  a.slice = ((vecs + parts - 1) / parts + 7) / 8 * 8 * VE;
+  const int per = a.slice / VE;
   const int threads = per >= 2048 ? 512 : per >= 512 ? 256 : 128;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.rows * parts));
-  cfg.blockDim = dim3(threads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, distill_kernel<T, MODE>, a);
+  return launch(distill_split_kernel<T, MODE>, a, a.rows * parts, threads, entries, parts, after, stream);
 }
 
 template <int MODE>
@@ -398,25 +962,36 @@ static int distill_run(const lpmm_b200_distill* d, void* stream_) {
   a.temperature = d->temperature;
   a.c = (float)(1.4426950408889634 / (double)d->temperature);
   a.scale = d->grad_scale;
+  a.grad_outer_stride = d->grad_outer_stride, a.grad_inner_stride = d->grad_inner_stride;
+  a.k_pad = (a.k + 3) / 4 * 4;
+  if (MODE != DISTILL_LOSS)
+    for (a.hash_size = 32; a.hash_size < 2 * a.k;) a.hash_size *= 2;
   if (d->rows == 0) {
     if (MODE != DISTILL_GRAD && !none) LPMM_CUDA_TRY(cudaMemsetAsync(d->loss, 0, sizeof(float), stream));
     return LPMM_B200_OK;
   }
-  if (MODE == DISTILL_BOTH && mean) {
+  const bool first = MODE == DISTILL_BOTH && mean;
+  if (first) {
     distill_reduce_kernel<<<1, 1024, 0, stream>>>(nullptr, d->weights, d->rows, 1, nullptr, norm);
     LPMM_CUDA_TRY(cudaGetLastError());
   }
   cudaError_t e;
   if (d->dtype == LPMM_B200_DTYPE_FP32)
-    e = distill_launch<float, MODE>(a, stream);
+    e = distill_launch<float, MODE>(a, first, stream);
   else if (d->dtype == LPMM_B200_DTYPE_BF16)
-    e = distill_launch<__nv_bfloat16, MODE>(a, stream);
+    e = distill_launch<__nv_bfloat16, MODE>(a, first, stream);
   else
-    e = distill_launch<__half, MODE>(a, stream);
+    e = distill_launch<__half, MODE>(a, first, stream);
   LPMM_CUDA_TRY(e);
   if (MODE != DISTILL_GRAD && !none) {
-    distill_reduce_kernel<<<1, 1024, 0, stream>>>(a.row_loss, d->weights, d->rows, mean, d->loss, norm);
-    LPMM_CUDA_TRY(cudaGetLastError());
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(1), cfg.blockDim = dim3(1024), cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    const float *row_loss = a.row_loss, *weights = d->weights;
+    LPMM_CUDA_TRY(cudaLaunchKernelEx(&cfg, distill_reduce_kernel, row_loss, weights, (long long)d->rows, (int)mean, d->loss, norm));
   }
   return LPMM_B200_OK;
 }

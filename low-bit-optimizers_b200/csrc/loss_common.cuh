@@ -15,6 +15,17 @@ struct Elem<float> {
   static constexpr int VE = 4;
   static __device__ __forceinline__ float widen(float v) { return v; }
   static __device__ __forceinline__ float narrow(float v) { return v; }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+  template <int N>
+  static __device__ __forceinline__ float maximum(const uint4* u) {  // NaN is passed over, here and below
+    float m = __uint_as_float(u[0].x);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      m = fmaxf(m, fmaxf(__uint_as_float(u[j].x), __uint_as_float(u[j].y)));
+      m = fmaxf(m, fmaxf(__uint_as_float(u[j].z), __uint_as_float(u[j].w)));
+    }
+    return m;
+  }
   static __device__ __forceinline__ void unpack(const uint4& r, float* x) {
     x[0] = __uint_as_float(r.x), x[1] = __uint_as_float(r.y), x[2] = __uint_as_float(r.z), x[3] = __uint_as_float(r.w);
   }
@@ -27,6 +38,16 @@ struct Elem<__nv_bfloat16> {
   static constexpr int VE = 8;
   static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+  template <int N>
+  static __device__ __forceinline__ float maximum(const uint4* u) {
+    __nv_bfloat162 m = as2(u[0].x);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      m = __hmax2(m, __hmax2(__hmax2(as2(u[j].x), as2(u[j].y)), __hmax2(as2(u[j].z), as2(u[j].w))));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ __nv_bfloat162 as2(uint32_t w) { return *reinterpret_cast<const __nv_bfloat162*>(&w); }
   static __device__ __forceinline__ void two(uint32_t w, float* x) {  // a bf16 is the upper half of its fp32 value
     x[0] = __uint_as_float(w << 16), x[1] = __uint_as_float(w & 0xffff0000u);
   }
@@ -46,6 +67,16 @@ struct Elem<__half> {
   static constexpr int VE = 8;
   static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
+  template <int N>
+  static __device__ __forceinline__ float maximum(const uint4* u) {
+    __half2 m = as2(u[0].x);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      m = __hmax2(m, __hmax2(__hmax2(as2(u[j].x), as2(u[j].y)), __hmax2(as2(u[j].z), as2(u[j].w))));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+  static __device__ __forceinline__ __half2 as2(uint32_t w) { return *reinterpret_cast<const __half2*>(&w); }
   static __device__ __forceinline__ void two(uint32_t w, float* x) {
     const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
     x[0] = f.x, x[1] = f.y;
@@ -79,6 +110,55 @@ __device__ __forceinline__ float load_any(const void* p, long long i, int dtype)
 __device__ __forceinline__ long long load_index(const void* p, long long i, int bits) {
   return bits == 64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
+
+// ---------------------------------------------------------------------------------------------
+// barriers in shared memory and bulk copies into it
+// ---------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mbar_init(unsigned long long* b, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_at(b)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mbar_arrive(unsigned long long* b) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_at(b)) : "memory");
+}
+__device__ __forceinline__ void mbar_expect(unsigned long long* b, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(b)), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool mbar_test(unsigned long long* b, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_at(b)), "r"(parity)
+      : "memory");
+  return done;
+}
+constexpr int WAIT_LIMIT = 1 << 22;  // tries, each of which may sleep for a while: seconds, where a wait is microseconds
+// Waits for the phase; gives up when the limit is reached or another thread of the CTA has given up (*failed).  The
+// caller goes on in either case (its data are then worthless, its accesses in range) and the kernel ends as it should.
+__device__ __forceinline__ void mbar_wait(unsigned long long* b, uint32_t parity, int* failed) {
+  if (mbar_test(b, parity)) return;
+  for (int i = 0; i < WAIT_LIMIT; ++i) {
+    if (mbar_test(b, parity) || *(volatile int*)failed) return;
+  }
+  *(volatile int*)failed = 1;
+}
+__device__ __forceinline__ void mbar_wait_landed(unsigned long long* b, uint32_t parity) {
+  for (int i = 0; i < WAIT_LIMIT; ++i)
+    if (mbar_test(b, parity)) return;
+}
+// both addresses and the size are multiples of 16 bytes
+__device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, unsigned long long* b) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_at(to)),
+               "l"(from), "r"(bytes), "r"(smem_at(b))
+               : "memory");
+}
+
+// A kernel launched with launch_after(): waits until the kernel before it has finished and its results can be read.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// lets a kernel launched with launch_after() start (it still waits for this one's end in pdl_wait)
+__device__ __forceinline__ void pdl_start_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 __device__ __forceinline__ float nan_f() { return __int_as_float(0x7fc00000); }
 

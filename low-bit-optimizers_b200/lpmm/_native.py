@@ -61,7 +61,8 @@ class StepTensor(ctypes.Structure):
 class Distill(ctypes.Structure):
     """``lpmm_b200_distill``"""
     _fields_ = ([(n, ctypes.c_void_p) for n in ("logits", "grad", "teacher", "index", "weights", "upstream", "loss", "work")]
-                + [(n, ctypes.c_int64) for n in ("rows", "inner", "outer_stride", "inner_stride", "vocab", "k")]
+                + [(n, ctypes.c_int64) for n in ("rows", "inner", "outer_stride", "inner_stride", "grad_outer_stride",
+                                                 "grad_inner_stride", "vocab", "k")]
                 + [(n, ctypes.c_int32) for n in ("dtype", "teacher_dtype", "index_bits", "reduction")]
                 + [("temperature", ctypes.c_float), ("grad_scale", ctypes.c_float)])
 

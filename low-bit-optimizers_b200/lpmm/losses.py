@@ -45,8 +45,35 @@ def _row_strides(t):
         if t.dim() == 2:
             return t, 1, t.stride(0), 0
         if t.dim() == 3:
-            return t, max(t.shape[1], 1), t.stride(0), t.stride(1)
+            return (t, t.shape[1], t.stride(0), t.stride(1)) if t.shape[1] > 1 else (t, 1, t.stride(0), 0)
     return t.contiguous(), 1, n, 0
+
+
+def _grad_of(logits, d):
+    """A tensor for the gradient of ``logits`` (the tensor that ``d`` describes), its strides in ``d``.  Contiguous where
+    that puts every row to the 16-byte boundaries as the logits' row lies to them, which the kernels' wide accesses
+    need; else with up to 16 bytes between rows."""
+    n, size = logits.shape[-1], logits.element_size()
+    off, wide = logits.data_ptr() % 16 // size, 16 // size
+    if d.inner == 1:
+        inner, outer = 0, n + (d.outer_stride - n) % wide
+        odd = outer != n
+    else:
+        inner = n + (d.inner_stride - n) % wide
+        outer = d.inner * inner + (d.outer_stride - d.inner * inner) % wide
+        odd = inner != n or outer != d.inner * n
+    if off or odd:
+        rows = -(-d.rows // d.inner)
+        grad = torch.empty(off + rows * outer, dtype=logits.dtype, device=logits.device)
+        if odd:  # two or three axes: others are contiguous
+            strides = (outer, 1) if logits.dim() == 2 else (outer, inner or n, 1)
+            grad = grad.as_strided(logits.shape, strides, off)
+        else:
+            grad = grad[off:].view(logits.shape)
+    else:
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    d.grad, d.grad_outer_stride, d.grad_inner_stride = grad.data_ptr(), outer, inner
+    return grad
 
 
 def _launch(fn, args, device):
@@ -124,9 +151,9 @@ class _TopkDistillation(torch.autograd.Function):
         temperature, reduction = ctx.how
         with torch.no_grad():
             d, kept, rows, lead = _distill_args(logits, teacher_logits, teacher_idx, temperature, weights, reduction)
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = _grad_of(kept[0], d)
         upstream = upstream.to(torch.float32).contiguous()
-        d.grad, d.work, d.upstream = grad.data_ptr(), ctx.work.data_ptr(), upstream.data_ptr()
+        d.work, d.upstream = ctx.work.data_ptr(), upstream.data_ptr()
         _launch(N.lib.lpmm_b200_distill_backward, d, logits.device)
         return grad, None, None, None, None, None
 
@@ -162,12 +189,13 @@ def topk_distillation_with_grad(logits, teacher_logits, teacher_idx, temperature
     """``topk_distillation`` and its gradient in one call: ``(loss, grad)``.
 
     ``grad`` is ``grad_scale`` (a loss scale, a share of the total loss) times the derivative of the loss by ``logits``,
-    of the losses' sum with ``reduction="none"``: a new contiguous tensor of the logits' shape and type, for
-    ``logits.backward(grad)``.  ``loss`` is not scaled, and neither takes part in autograd."""
+    of the losses' sum with ``reduction="none"``: a new tensor of the logits' shape and type, for ``logits.backward(grad)``
+    (contiguous, but with up to 16 bytes between rows where the logits' rows lie to the 16-byte boundaries in another way
+    than a contiguous tensor's would).  ``loss`` is not scaled, and neither takes part in autograd."""
     d, kept, rows, lead = _distill_args(logits, teacher_logits, teacher_idx, temperature, weights, reduction)
     loss, work = _distill_outputs(d, rows, lead, logits.device)
-    grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    d.grad, d.grad_scale = grad.data_ptr(), float(grad_scale)
+    grad = _grad_of(kept[0], d)
+    d.grad_scale = float(grad_scale)
     _launch(N.lib.lpmm_b200_distill_forward_backward, d, logits.device)
     return loss, grad
 

@@ -86,7 +86,8 @@ def check_distill(x, t, idx, temp=1.0, w=None, reduction="sum", scale=1.0, grad_
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("rows, vocab, k", [
     (1, 1, 1), (3, 2, 2), (5, 7, 3), (4, 8, 1), (3, 9, 4), (2, 31, 5), (7, 128, 16), (40, 1000, 64), (3, 4097, 33),
-    (2, 32000, 64), (3, 50257, 100), (1, 131075, 1024), (300, 515, 9), (1, 3, 7), (700, 260, 300),
+    (2, 32000, 64), (3, 50257, 100), (1, 131075, 1024), (300, 515, 9), (1, 3, 7), (700, 260, 300), (5, 2048, 256), (9, 2049, 257),
+    (33, 8192, 40), (6, 8193, 1000), (3, 1024, 31), (310, 8200, 12), (640, 16391, 65), (200, 40003, 1024), (160, 70001, 33),
 ])
 def test_distillation_sizes(dtype, rows, vocab, k):
     x, t, idx = distill_inputs(rows, vocab, k, dtype, seed=rows + vocab)

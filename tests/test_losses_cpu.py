@@ -104,6 +104,7 @@ def test_balance_refuses(host, what, change, error, text):
 
 def _rows_of(t, inner, outer, step):
     """First elements of the rows that the layout names, read from the storage."""
+    inner = max(inner, 1)
     flat = t.as_strided((t.untyped_storage().nbytes() // t.element_size(),), (1,), 0)
     rows = t.numel() // t.shape[-1]
     at = [t.storage_offset() + (r // inner) * outer + (r % inner) * step for r in range(rows)]
@@ -131,6 +132,31 @@ def test_row_layout(make, copied):
     got, inner, outer, step = L._row_strides(t)
     assert (got is not t) == copied and inner >= 1
     assert torch.equal(_rows_of(got, inner, outer, step), t.reshape(-1, t.shape[-1])[:, 0])
+
+
+@pytest.mark.parametrize("make", [
+    lambda b: b, lambda b: b[:, :-1], lambda b: b[:, 1:], lambda b: b[..., :-3], lambda b: b[..., 1:], lambda b: b.transpose(0, 1),
+    lambda b: b[0, 0].expand(4, 5, 203), lambda b: b.transpose(1, 2), lambda b: b[:, ::2, 3:], lambda b: b[None],
+    lambda b: b[1, 2], lambda b: b[:, 1], lambda b: b[:0], lambda b: b[:, :1, 5:6], lambda b: b.reshape(-1)[1:].view(1, -1),
+    lambda b: b.transpose(0, 1)[:, 1:],
+])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_layout(make, dtype):
+    """The gradient's rows are where the structure says, apart, inside their storage, and like the logits' rows to 16 bytes."""
+    t = make(torch.zeros(4, 5, 203, dtype=dtype))
+    got, inner, outer, step = L._row_strides(t)
+    d = N.Distill(inner=inner, outer_stride=outer, inner_stride=step, rows=got.numel() // got.shape[-1])
+    g = L._grad_of(got, d)
+    assert g.shape == t.shape and g.dtype == dtype
+    flat = g.as_strided((g.untyped_storage().nbytes() // g.element_size(),), (1,), 0).fill_(-1)
+    g.copy_((torch.arange(g.numel()) % 251).view(g.shape))
+    assert torch.equal(g.reshape(-1).float(), torch.arange(g.numel()).remainder(251).float())
+    assert torch.equal(_rows_of(g, inner, d.grad_outer_stride, d.grad_inner_stride), g.reshape(-1, g.shape[-1])[:, 0])
+    wide = 16 // t.element_size()
+    if d.rows:
+        assert d.grad == g.data_ptr() and (got.data_ptr() - d.grad) % 16 == 0
+    assert (outer - d.grad_outer_stride) % wide == 0 and (step - d.grad_inner_stride) % wide == 0
+    assert flat.numel() <= g.numel() + wide * (d.rows + 2 + d.rows // max(inner, 1))
 
 
 def test_structures_as_the_library_gets_them(host):
@@ -169,6 +195,12 @@ def test_library_refuses_bad_arguments_before_any_launch():
     at = ctypes.addressof(some)
     d = N.Distill(**dict(good, logits=at, grad=at, teacher=at, index=at, upstream=at, loss=at, work=(at + 15) // 16 * 16 + 4))
     assert all(fn(ref(d), None) == -2 for fn in forms)
+    # a gradient that lies otherwise to the 16-byte boundaries than the logits
+    room = (at + 15) // 16 * 16
+    for change in (dict(grad=room + 4), dict(grad_outer_stride=9)):
+        d = N.Distill(**dict(dict(good, logits=room, grad=room, teacher=at, index=at, upstream=at, loss=at, work=room,
+                                  grad_outer_stride=8), **change))
+        assert all(fn(ref(d), None) == -2 for fn in forms[1:])
     forms = (lib.lpmm_b200_balance_forward, lib.lpmm_b200_balance_backward, lib.lpmm_b200_balance_forward_backward)
     good = dict(tokens=1, inner=1, outer_stride=8, experts=8, k=1, sequences=1, index_bits=64)
     for fn in forms:
