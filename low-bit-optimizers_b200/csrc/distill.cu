@@ -9,10 +9,12 @@
 // K entries are written over it.  All sums are fp32, the gradient is rounded once.  Exponentials are 2^(x c - M) with
 // c = log2(e) / T and M = RN(m c), one fma and one hardware exponential each.
 // Three kernels, by the size of the problem (distill_launch):
-//   small   a row in the registers of one warp or of 128 threads
-//   stream  persistent CTAs, rows through a ring of shared memory filled by bulk copies
-//   split   a row's columns shared by a cluster of CTAs, for few rows
+//   rows    rows of up to 16 KB: every warp takes rows of its own, copied into shared memory some rows ahead
+//   stream  larger rows: persistent CTAs (or clusters that share a row's columns), a ring of bulk copies
+//   split   few rows: one CTA or one cluster per row
 #include <cooperative_groups.h>
+
+#include <atomic>
 
 #include "loss_common.cuh"
 
@@ -44,9 +46,11 @@ struct DistillArgs {
   int vocab, k, teacher_dtype, index_bits, upstream_per_row;
   float temperature, c;  // c = log2(e) / T
   float scale;
-  int slice;             // split: columns per CTA of the cluster
+  int slice;             // stream, split: columns per CTA of the cluster
   int k_pad, hash_size;  // entries per row rounded up, slots of the table that finds an index given twice
-  int stages, resident;  // stream: chunks in the ring; a row stays in it for both passes
+  int stages, resident;  // stream: chunks in the ring; a row stays in it for both passes.  rows: rows ahead per warp
+  int slot;              // rows: bytes of a row in shared memory
+  int tellers;           // stream: warps that prepare entries
 };
 
 constexpr float LOWEST = -3.402823466e38f;
@@ -238,16 +242,36 @@ struct Block {  // all threads of the CTA (at most 16 warps)
 
 struct Entries {
   int* idx;    // [k_pad], -1: no entry
-  float* p;    // [k_pad] t - tm, then the probability
+  float* z;    // [k_pad] (t - tm) c: the probability is 2^z / ts
   float* x;    // [k_pad] the student's logit
   int* hash;   // [hash_size], -1 when not in use
   int* twice;  // an index occurs more than once
 };
 
+__host__ __device__ constexpr size_t entry_bytes(int k_pad, int hash_size) { return 12 * (size_t)k_pad + 4 * (size_t)hash_size; }
+
+__device__ __forceinline__ Entries entries_at(char* p, const DistillArgs& a, int* twice) {
+  Entries e;
+  e.idx = reinterpret_cast<int*>(p);
+  e.z = reinterpret_cast<float*>(p + 4 * a.k_pad);
+  e.x = reinterpret_cast<float*>(p + 8 * a.k_pad);
+  e.hash = reinterpret_cast<int*>(p + 12 * a.k_pad);
+  e.twice = twice;
+  return e;
+}
+
 struct Teacher {
   float w, tm, ts;
   bool live;  // weight and entries: the row has a part in the loss
 };
+
+// puts i into the table; true if it was there
+__device__ __forceinline__ bool seen(int* hash, int size, int i) {
+  for (unsigned h = ((unsigned)i * 2654435761u) >> 12;; ++h) {  // ends: the table is at most half full
+    const int was = atomicCAS(&hash[h & (size - 1)], -1, i);
+    if (was == -1 || was == i) return was == i;
+  }
+}
 
 // Reads the row's entries.  GRAD: the statistics are in `st`.  The team's threads may read `e` afterwards.
 template <typename T, int MODE, typename Team>
@@ -258,6 +282,7 @@ __device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, 
   t.tm = LOWEST;
   bool any = false, bad = false;
   if (team.rank() == 0) *e.twice = 0;
+#pragma unroll 2
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const long long i = load_index(a.index, row * a.k + k, a.index_bits);
     const float v = load_any(a.teacher, row * a.k + k, a.teacher_dtype);
@@ -266,73 +291,71 @@ __device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, 
     bad |= entry && !in;
     any |= entry;
     e.idx[k] = in ? (int)i : -1;
-    e.p[k] = v;
-    if (in && t.w != 0.0f) e.x[k] = Elem<T>::widen(x[i]);
+    e.z[k] = v;
+    if (in) e.x[k] = Elem<T>::widen(x[i]);
     if (entry) t.tm = fmaxf(t.tm, v);
   }
   t.live = team.any(any) && t.w != 0.0f;
   t.ts = 0.0f;
   if (!t.live) return t;
-  if (MODE == DISTILL_GRAD) {
+  if (MODE == DISTILL_GRAD)
     t.tm = st.tm;
-    t.ts = st.ts;
-  } else {
+  else
     t.tm = team.max(t.tm);
-    float sum = 0.0f;
-    for (int k = team.rank(); k < a.k; k += team.size())
-      if (e.idx[k] >= 0) sum += ex2((e.p[k] - t.tm) * a.c);
+  float sum = 0.0f;
+  for (int k = team.rank(); k < a.k; k += team.size()) {
+    const int i = e.idx[k];
+    const float z = (e.z[k] - t.tm) * a.c;
+    e.z[k] = z;
+    if (i < 0) continue;
+    sum += ex2(z);
+    if (MODE != DISTILL_LOSS && seen(e.hash, a.hash_size, i)) *e.twice = 1;
+  }
+  if (MODE == DISTILL_GRAD) {
+    t.ts = st.ts;
+    team.sync();
+  } else {
     t.ts = team.sum(sum);
     if (team.any(bad)) t.ts = nan_f();
   }
-  for (int k = team.rank(); k < a.k; k += team.size()) {
-    const int i = e.idx[k];
-    e.p[k] = i >= 0 ? ex2((e.p[k] - t.tm) * a.c) / t.ts : 0.0f;
-    if (MODE != DISTILL_LOSS && i >= 0) {
-      for (unsigned h = ((unsigned)i * 2654435761u) >> 12;; ++h) {  // ends: the table is at most half full
-        const int was = atomicCAS(&e.hash[h & (a.hash_size - 1)], -1, i);
-        if (was == i) *e.twice = 1;
-        if (was == -1 || was == i) break;
-      }
-    }
-  }
-  team.sync();
-  if (MODE != DISTILL_LOSS)
+  if (MODE != DISTILL_LOSS) {
     for (int i = team.rank(); i < a.hash_size; i += team.size()) e.hash[i] = -1;
+    team.sync();
+  }
   return t;
 }
 
-// sum_k p_k (log p_k - log q_k) of a prepared row, for all threads of the team.  log p_k from the probability itself
-// would lose the small ones: ln p = z ln2 with z = log2 p is read off p's own exponent argument, (t - tm) c - log2 ts.
+// sum_k p_k (log p_k - log q_k) of a prepared row, for all threads of the team: log2 p_k = z - log2 ts
 template <typename Team>
-__device__ __forceinline__ float divergence(const DistillArgs& a, long long row, const Teacher& t, Entries e, Team& team,
+__device__ __forceinline__ float divergence(const DistillArgs& a, const Teacher& t, const Entries& e, Team& team,
                                             const Expo& ex, float s) {
   float sum = 0.0f;
   for (int k = team.rank(); k < a.k; k += team.size()) {
-    const float p = e.p[k];
+    const float z = e.z[k], p = ex2(z);
     if (e.idx[k] < 0 || p == 0.0f) continue;
-    const float z = (load_any(a.teacher, row * a.k + k, a.teacher_dtype) - t.tm) * a.c;
     sum += p * (z - ex.log2_of(e.x[k]));
   }
-  return LN2 * team.sum(sum) + (logf(s) - logf(t.ts));
+  return LN2 * (team.sum(sum) / t.ts) + (logf(s) - logf(t.ts));
 }
 
 // The entries' columns within [lo, hi): q - p, written over q.  After a barrier behind the stores of q.
 template <typename T, typename Team>
 __device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const Entries& e, const Team& team,
-                                              const Expo& ex, float gs, float G, int lo, int hi) {
+                                              const Expo& ex, float gs, float G, float ts, int lo, int hi) {
   const bool twice = *e.twice;
+  const float Gp = G / ts;
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const int i = e.idx[k];
     if (i < lo || i >= hi) continue;
-    float p = e.p[k];
+    float p = ex2(e.z[k]);
     if (twice) {  // an index that occurs several times: its first entry writes for all, in their order
       bool first = true;
       for (int j = 0; j < k; ++j) first &= e.idx[j] != i;
       if (!first) continue;
       for (int j = k + 1; j < a.k; ++j)
-        if (e.idx[j] == i) p += e.p[j];
+        if (e.idx[j] == i) p += ex2(e.z[j]);
     }
-    g[i] = Elem<T>::narrow(gs * ex(e.x[k]) - G * p);
+    g[i] = Elem<T>::narrow(gs * ex(e.x[k]) - Gp * p);
   }
 }
 
@@ -351,108 +374,255 @@ __device__ __noinline__ float far_sum(const DistillArgs& a, const T* x, int lo, 
 }
 
 // ---------------------------------------------------------------------------------------------
-// small: a row in the registers of GT threads, all of its loads in flight at once
+// rows: every warp takes rows of its own; their logits are copied into its slots of shared memory some rows ahead, the
+// entries of the next row are loaded into registers (KV per lane)
 // ---------------------------------------------------------------------------------------------
-constexpr int SMALL_VECS = 8;
+constexpr int ROWS_MAX_WARPS = 8, ROWS_MAX_STAGES = 4, ROWS_MAX_BYTES = 16384;
 
-__host__ __device__ constexpr size_t entry_bytes(int k_pad, int hash_size) { return 12 * (size_t)k_pad + 4 * (size_t)hash_size; }
-
-__device__ __forceinline__ Entries entries_at(char* p, const DistillArgs& a, int* twice) {
-  Entries e;
-  e.idx = reinterpret_cast<int*>(p);
-  e.p = reinterpret_cast<float*>(p + 4 * a.k_pad);
-  e.x = reinterpret_cast<float*>(p + 8 * a.k_pad);
-  e.hash = reinterpret_cast<int*>(p + 12 * a.k_pad);
-  e.twice = twice;
-  return e;
-}
-
-template <typename T, int MODE, typename Team>
-__device__ __forceinline__ void small_row(const DistillArgs& a, long long row, Entries e, Team& team) {
-  using E = Elem<T>;
-  const T* x = logits_row<T>(a, row);
-  const Span o = span_of(x, 0, a.vocab);
-  const int t = team.rank();
-  const bool skip = a.weights && a.weights[row] == 0.0f;
-  uint4 u[SMALL_VECS];
-  const uint4* xv = reinterpret_cast<const uint4*>(x + o.head);
-#pragma unroll
-  for (int j = 0; j < SMALL_VECS; ++j) {
-    const int i = t + j * team.size();
-    u[j] = i < o.vecs && !skip ? xv[i] : E::none();
-  }
-  const int at = edge_of<T>(o, t);
-  const float edge = at >= 0 && !skip ? E::widen(x[at]) : -__int_as_float(0x7f800000);
-  RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-  if (MODE == DISTILL_GRAD) st = a.stats[row];
-  const Teacher tch = prepare<T, MODE>(a, row, x, e, team, st);
-  if (MODE != DISTILL_GRAD) {
-    Running r{LOWEST, 0.0f};
-    take<T, SMALL_VECS>(r, u, a.c);
-    take_one(r, edge, a.c);
-    r = team.joined(r, a.c);
-    st.m = r.m;
-    st.s = r.s;
-    if (tch.live && far_off(r.m, a.c)) {
-      st.s = far_sum(a, x, 0, a.vocab, r.m, team);
-      if (st.s == 0.0f) st.s = nan_f();  // every logit -inf: no distribution
-    }
-  }
-  const Expo ex(st.m, a.c);
-  if (MODE != DISTILL_GRAD) {
-    const float d = tch.live ? divergence(a, row, tch, e, team, ex, st.s) : 0.0f;
-    if (t == 0) {
-      a.row_loss[row] = tch.live ? tch.w * a.temperature * a.temperature * d : 0.0f;
-      a.stats[row] = RowStats{st.m, st.s, tch.tm, tch.ts};
-    }
-  }
-  if (MODE == DISTILL_LOSS) return;
-  T* g = grad_row<T>(a, row);
-  uint4* gv = reinterpret_cast<uint4*>(g + o.head);
-  const float G = tch.live ? upstream_of(a, row) * tch.w * a.temperature + (tch.ts - tch.ts) : 0.0f;
-  const float gs = tch.live ? G / st.s : 0.0f;
-#pragma unroll
-  for (int j = 0; j < SMALL_VECS; ++j) {
-    const int i = t + j * team.size();
-    if (i < o.vecs) gv[i] = tch.live ? ex.scaled<T>(u[j], gs) : make_uint4(0, 0, 0, 0);
-  }
-  if (at >= 0) g[at] = E::narrow(tch.live ? gs * ex(edge) : 0.0f);
-  team.sync();
-  if (tch.live) write_entries(a, g, e, team, ex, gs, G, 0, a.vocab);
-}
-
-template <typename T, int MODE, int GT>
-__global__ void __launch_bounds__(128) distill_small_kernel(const DistillArgs a) {
-  extern __shared__ __align__(16) char smem[];
-  __shared__ float2 red[32];
-  __shared__ int twice[128 / GT];
-  const int mine = threadIdx.x / GT;
-  const long long row = (long long)blockIdx.x * (128 / GT) + mine;
-  const Entries e = entries_at(smem + mine * entry_bytes(a.k_pad, a.hash_size), a, &twice[mine]);
-  if (MODE != DISTILL_LOSS) {
-    for (int i = threadIdx.x % GT; i < a.hash_size; i += GT) e.hash[i] = -1;
-  }
-  pdl_wait();
-  if (GT == 32) {
-    __syncwarp();
+// What a warp loads of its next row, as it lies in memory: a conversion here would wait for the load.
+template <typename T, int MODE, int KV>
+struct RowFetch {
+  unsigned long long i_raw[KV];
+  uint32_t t_raw[KV], edge_raw;
+  float w, up;
+  RowStats st;
+  __device__ __forceinline__ void load(const DistillArgs& a, long long row) {
+    const int lane = threadIdx.x & 31;
     if (row >= a.rows) return;
-    Warp team;
-    small_row<T, MODE>(a, row, e, team);
-  } else {
-    __syncthreads();
-    Block team(red);
-    small_row<T, MODE>(a, row, e, team);
+    w = a.weights ? a.weights[row] : 1.0f;
+    const long long first = row * a.k;
+#pragma unroll
+    for (int j = 0; j < KV; ++j) {
+      const int k = lane + 32 * j;
+      i_raw[j] = ~0ull;
+      t_raw[j] = 0;
+      if (k < a.k) {
+        i_raw[j] = a.index_bits == 64 ? reinterpret_cast<const unsigned long long*>(a.index)[first + k]
+                                      : (unsigned long long)reinterpret_cast<const uint32_t*>(a.index)[first + k];
+        t_raw[j] = a.teacher_dtype == LPMM_B200_DTYPE_FP32 ? reinterpret_cast<const uint32_t*>(a.teacher)[first + k]
+                                                           : reinterpret_cast<const unsigned short*>(a.teacher)[first + k];
+      }
+    }
+    const T* x = logits_row<T>(a, row);
+    const int at = edge_of<T>(span_of(x, 0, a.vocab), lane);
+    edge_raw = Elem<T>::none().x;
+    if (at >= 0) edge_raw = Elem<T>::raw(x + at);
+    if (MODE == DISTILL_GRAD) {
+      st = a.stats[row];
+      up = a.upstream[a.upstream_per_row ? row : 0];
+    }
   }
+  __device__ __forceinline__ long long index(const DistillArgs& a, int j) const {
+    return a.index_bits == 64 ? (long long)i_raw[j] : (long long)(int)(uint32_t)i_raw[j];
+  }
+  __device__ __forceinline__ float teacher(const DistillArgs& a, int j) const {
+    if (a.teacher_dtype == LPMM_B200_DTYPE_FP32) return __uint_as_float(t_raw[j]);
+    if (a.teacher_dtype == LPMM_B200_DTYPE_BF16) return __uint_as_float(t_raw[j] << 16);
+    return __half2float(__ushort_as_half((unsigned short)t_raw[j]));
+  }
+  __device__ __forceinline__ float edge() const { return Elem<T>::of_raw(edge_raw); }
+};
+
+template <typename T, int MODE, int KV>
+__global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, 2) distill_rows_kernel(const DistillArgs a) {
+  using E = Elem<T>;
+  extern __shared__ __align__(16) char smem[];
+  __shared__ unsigned long long full[ROWS_MAX_WARPS][ROWS_MAX_STAGES];
+  __shared__ int failed;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  char* slots = smem + (size_t)warp * a.stages * a.slot;
+  int* hash = reinterpret_cast<int*>(smem + (size_t)warps * a.stages * a.slot) + warp * a.hash_size;
+  if (lane == 0) {
+    for (int i = 0; i < a.stages; ++i) mbar_init(&full[warp][i], 1);
+    mbar_fence();
+  }
+  if (threadIdx.x == 0) failed = 0;
+  if (MODE != DISTILL_LOSS)
+    for (int i = lane; i < a.hash_size; i += 32) hash[i] = -1;
+  __syncthreads();
+  const long long stride = (long long)gridDim.x * warps, row0 = (long long)blockIdx.x * warps + warp;
+  // bit i of `dead`: row number 32 n + i of this warp has weight 0 and is not copied; `dead_next`: of the next 32
+  auto weights_of = [&](long long it) {
+    const long long r = row0 + (it + lane) * stride;
+    return __ballot_sync(~0u, a.weights && r < a.rows && a.weights[r] == 0.0f);
+  };
+  uint32_t dead = weights_of(0), dead_next = weights_of(32);
+  auto copy = [&](long long it, int st, bool none) {
+    const long long row = row0 + it * stride;
+    if (lane != 0 || row >= a.rows) return;
+    const T* x = logits_row<T>(a, row);
+    const Span o = span_of(x, 0, a.vocab);
+    const uint32_t n = none ? 0 : o.vecs * 16;
+    mbar_expect(&full[warp][st], n);
+    if (n) bulk_load(slots + (size_t)st * a.slot, x + o.head, n, &full[warp][st]);
+  };
+  for (int i = 0; i < a.stages; ++i) copy(i, i, dead >> i & 1);
+  RowFetch<T, MODE, KV> next;
+  next.load(a, row0);
+  pdl_wait();
+  const float up0 = a.scale * (a.norm ? *a.norm : 1.0f);
+  int st = 0;
+  uint32_t phase = 0;
+  for (long long it = 0, row = row0; row < a.rows; ++it, row += stride) {
+    RowFetch<T, MODE, KV> f = next;
+    next.load(a, row + stride);
+    const T* x = logits_row<T>(a, row);
+    const Span o = span_of(x, 0, a.vocab);
+    const T* xs = reinterpret_cast<const T*>(slots + (size_t)st * a.slot);  // column head is its first
+    const uint4* buf = reinterpret_cast<const uint4*>(xs);
+    mbar_wait(&full[warp][st], phase, &failed);
+
+    // entries
+    int idx[KV];
+    float tk[KV], tm = LOWEST;
+    const float edge = f.edge();
+    bool any = false, bad = false;
+#pragma unroll
+    for (int j = 0; j < KV; ++j) {
+      const long long i = f.index(a, j);
+      tk[j] = f.teacher(a, j);
+      const bool entry = i >= 0 && tk[j] != -__int_as_float(0x7f800000);
+      const bool in = entry && i < a.vocab;  // an index outside of the vocabulary is not followed
+      bad |= entry && !in;
+      any |= entry;
+      idx[j] = in ? (int)i : -1;
+      if (entry) tm = fmaxf(tm, tk[j]);
+    }
+    const bool live = __any_sync(~0u, any) && f.w != 0.0f;
+    bad = __any_sync(~0u, bad);
+    float xk[KV];
+#pragma unroll
+    for (int j = 0; j < KV; ++j) {
+      const int i = idx[j];
+      xk[j] = 0.0f;
+      if (i >= 0 && live) xk[j] = E::widen(i >= o.head && i < o.tail_at ? xs[i - o.head] : x[i]);
+    }
+
+    // statistics
+    Running r{LOWEST, 0.0f};
+    float ts = 0.0f;
+    if (MODE != DISTILL_GRAD && live) {
+      for (int v = lane; v < o.vecs; v += 128) {
+        uint4 u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = v + 32 * j < o.vecs ? buf[v + 32 * j] : E::none();
+        take<T, 4>(r, u, a.c);
+      }
+      take_one(r, edge, a.c);
+      float m = r.m;
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+        tm = fmaxf(tm, __shfl_xor_sync(~0u, tm, d));
+      }
+      r.s *= ex2(ref_of(r.m, a.c) - ref_of(m, a.c));
+      r.m = m;
+    }
+    if (MODE == DISTILL_GRAD) tm = f.st.tm, ts = f.st.ts, r.m = f.st.m, r.s = f.st.s;
+    float z[KV], p[KV];
+#pragma unroll
+    for (int j = 0; j < KV; ++j) {
+      z[j] = (tk[j] - tm) * a.c;
+      p[j] = idx[j] >= 0 ? ex2(z[j]) : 0.0f;
+      if (MODE != DISTILL_GRAD) ts += p[j];
+    }
+    if (MODE != DISTILL_GRAD && live) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) {
+        r.s += __shfl_xor_sync(~0u, r.s, d);
+        ts += __shfl_xor_sync(~0u, ts, d);
+      }
+      if (bad) ts = nan_f();
+      if (far_off(r.m, a.c)) {
+        Warp team;
+        r.s = far_sum(a, x, 0, a.vocab, r.m, team);
+        if (r.s == 0.0f) r.s = nan_f();  // every logit -inf: no distribution
+      }
+    }
+    const Expo ex(r.m, a.c);
+    if (MODE != DISTILL_GRAD) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int j = 0; j < KV; ++j)
+        if (p[j] != 0.0f) sum += p[j] * (z[j] - ex.log2_of(xk[j]));
+      sum = Warp().sum(sum);
+      if (lane == 0) {
+        a.row_loss[row] = live ? f.w * a.temperature * a.temperature * (LN2 * (sum / ts) + (logf(r.s) - logf(ts))) : 0.0f;
+        a.stats[row] = RowStats{r.m, r.s, tm, ts};
+      }
+    }
+    if (MODE != DISTILL_LOSS) {
+      T* g = grad_row<T>(a, row);
+      uint4* gv = reinterpret_cast<uint4*>(g + o.head);
+      const int at = edge_of<T>(o, lane);
+      const float G = live ? up0 * (MODE == DISTILL_GRAD ? f.up : 1.0f) * f.w * a.temperature + (ts - ts) : 0.0f;
+      const float gs = G / r.s, Gp = G / ts;
+      if (live) {
+        for (int v = lane; v < o.vecs; v += 32) gv[v] = ex.scaled<T>(buf[v], gs);
+        if (at >= 0) g[at] = E::narrow(gs * ex(edge));
+        bool twice = false;
+#pragma unroll
+        for (int j = 0; j < KV; ++j)
+          if (idx[j] >= 0) twice |= seen(hash, a.hash_size, idx[j]);
+        __syncwarp();
+        for (int i = lane; i < a.hash_size; i += 32) hash[i] = -1;
+        bool mine[KV];
+#pragma unroll
+        for (int j = 0; j < KV; ++j) mine[j] = idx[j] >= 0;
+        if (__any_sync(~0u, twice)) {  // an index that occurs several times: its first entry writes for all, in their order
+          float all[KV];
+#pragma unroll
+          for (int j = 0; j < KV; ++j) all[j] = 0.0f;
+#pragma unroll
+          for (int q = 0; q < KV; ++q)
+            for (int l = 0; l < 32; ++l) {
+              const int other = __shfl_sync(~0u, idx[q], l);
+              const float po = __shfl_sync(~0u, p[q], l);
+#pragma unroll
+              for (int j = 0; j < KV; ++j)
+                if (other == idx[j]) {
+                  all[j] += po;
+                  if (q * 32 + l < j * 32 + lane) mine[j] = false;
+                }
+            }
+#pragma unroll
+          for (int j = 0; j < KV; ++j) p[j] = all[j];
+        }
+#pragma unroll
+        for (int j = 0; j < KV; ++j)
+          if (mine[j]) g[idx[j]] = E::narrow(gs * ex(xk[j]) - Gp * p[j]);
+      } else {
+        for (int v = lane; v < o.vecs; v += 32) gv[v] = make_uint4(0, 0, 0, 0);
+        if (at >= 0) g[at] = E::narrow(0.0f);
+      }
+    }
+    __syncwarp();
+    if ((it & 31) == 31) {
+      dead = dead_next;
+      dead_next = weights_of(it + 33);
+    }
+    // row number it + stages takes the slot; its bit is in the current word (which from here on is that of it + 1) or the next
+    const int ahead = (int)((it + 1) & 31) + a.stages - 1;
+    copy(it + a.stages, st, (ahead < 32 ? dead >> ahead : dead_next >> (ahead - 32)) & 1);
+    if (++st == a.stages) st = 0, phase ^= 1;
+  }
+  __syncthreads();
+  if (failed)  // a wait ran out (it never has): what this CTA wrote is not to be taken for a result
+    for (long long row = row0; row < a.rows; row += stride)
+      if (lane == 0) {
+        if (MODE != DISTILL_GRAD) a.row_loss[row] = nan_f();
+        if (MODE != DISTILL_LOSS) grad_row<T>(a, row)[0] = E::narrow(nan_f());
+      }
 }
 
 // ---------------------------------------------------------------------------------------------
-// stream: persistent CTAs; one warp copies the rows into a ring of chunks, one prepares the entries of the next row,
-// eight take the passes
+// stream: persistent CTAs, or clusters of them that share the columns of a row; one warp copies the rows into a ring of
+// chunks, a few prepare the entries of the next rows, eight take the passes
 // ---------------------------------------------------------------------------------------------
 constexpr int CHUNK = 8192;
 constexpr int CWARPS = 8, CTHREADS = CWARPS * 32;
 constexpr int PER = CHUNK / 16 / CTHREADS;  // vectors per thread and chunk
-constexpr int MAX_STAGES = 28;
+constexpr int MAX_STAGES = 14, MAX_TELLERS = 4, MAX_PARTS = 8;
 
 struct StreamRow {  // what the consumers are told about a row, and what they tell
   Teacher t;
@@ -462,8 +632,11 @@ struct StreamRow {  // what the consumers are told about a row, and what they te
 
 struct StreamSmem {
   unsigned long long full[MAX_STAGES], empty[MAX_STAGES];
-  unsigned long long told[2], freed[2], stat[2];  // entries ready / no longer read / statistics of the row known
-  StreamRow row[2];
+  // per slot: entries ready / no longer read / statistics of the row known
+  unsigned long long told[MAX_TELLERS], freed[MAX_TELLERS], stat[MAX_TELLERS];
+  unsigned long long joined[2];  // the statistics of all parts of a row are in `part`
+  float2 part[2][MAX_PARTS];
+  StreamRow row[MAX_TELLERS];
   float2 red[2][CWARPS];
   int failed;
 };
@@ -488,45 +661,59 @@ struct Consumers {
     for (int i = 1; i < CWARPS; ++i) v += r[i].x;
     return v;
   }
-  __device__ __forceinline__ Running joined(Running v, float c) {
-    v = warp_join(v, c);
-    const float2 o = exchange(make_float2(v.m, v.s))[threadIdx.x % CWARPS];
+  // of n <= 8 values that lanes 0 ... n - 1, repeated over the warp, hold
+  static __device__ __forceinline__ Running join_of(float2 o, int n, float c) {
     float m = o.x;
 #pragma unroll
-    for (int d = CWARPS / 2; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+    for (int d = 4; d; d >>= 1)
+      if (d < n) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
     float s = o.y * ex2(ref_of(o.x, c) - ref_of(m, c));
 #pragma unroll
-    for (int d = CWARPS / 2; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
+    for (int d = 4; d; d >>= 1)
+      if (d < n) s += __shfl_xor_sync(~0u, s, d);
     return Running{m, s};
+  }
+  __device__ __forceinline__ Running joined(Running v, float c) {
+    v = warp_join(v, c);
+    return join_of(exchange(make_float2(v.m, v.s))[threadIdx.x % CWARPS], CWARPS, c);
   }
 };
 
 template <typename T, int MODE>
-__global__ void __launch_bounds__(CTHREADS + 64, 2) distill_stream_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_stream_kernel(const DistillArgs a) {
   using E = Elem<T>;
   extern __shared__ __align__(16) char smem[];
   char* ring = smem;
   StreamSmem& sm = *reinterpret_cast<StreamSmem*>(smem + (size_t)a.stages * CHUNK);
   char* entry_mem = smem + (size_t)a.stages * CHUNK + (sizeof(StreamSmem) + 15) / 16 * 16;
-  const size_t per_slot = 12 * (size_t)a.k_pad;
+  const size_t per_slot = entry_bytes(a.k_pad, a.hash_size);
+  cg::cluster_group cluster = cg::this_cluster();
+  const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
+  const int lo = min(part * a.slice, a.vocab), hi = min(lo + a.slice, a.vocab);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(&sm.full[i], 1);
       mbar_init(&sm.empty[i], CWARPS);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < a.tellers; ++i) {
       mbar_init(&sm.told[i], 1);
       mbar_init(&sm.freed[i], CWARPS);
       mbar_init(&sm.stat[i], 1);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(&sm.joined[i], 1);
     sm.failed = 0;
     mbar_fence();
   }
-  int* hash = reinterpret_cast<int*>(entry_mem + 2 * per_slot);
-  for (int i = threadIdx.x; i < a.hash_size; i += blockDim.x) hash[i] = -1;
-  __syncthreads();
-  const long long grid = gridDim.x;
+  for (int j = 0; j < a.tellers; ++j) {
+    int* hash = entries_at(entry_mem + j * per_slot, a, nullptr).hash;
+    for (int i = threadIdx.x; i < a.hash_size; i += blockDim.x) hash[i] = -1;
+  }
+  if (parts > 1)
+    cluster.sync();
+  else
+    __syncthreads();
+  const long long grid = gridDim.x / parts, row0 = blockIdx.x / parts;
   // passes over the chunks: once where the row stays in the ring, or only one pass is made
   const int loads = MODE == DISTILL_BOTH && !a.resident ? 2 : 1;
 
@@ -534,7 +721,7 @@ __global__ void __launch_bounds__(CTHREADS + 64, 2) distill_stream_kernel(const 
     int st = 0, fills = 0;
     uint32_t phase = 0, skips = 0;
     long long it = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += grid, ++it) {
+    for (long long row = row0; row < a.rows; row += grid, ++it) {
       if ((it & 31) == 0) {
         const long long r = row + lane * grid;
         skips = __ballot_sync(~0u, a.weights && r < a.rows && a.weights[r] == 0.0f);
@@ -542,8 +729,8 @@ __global__ void __launch_bounds__(CTHREADS + 64, 2) distill_stream_kernel(const 
       if (skips >> (it & 31) & 1) continue;
       if (lane == 0) {
         const T* x = logits_row<T>(a, row);
-        const Span o = span_of(x, 0, a.vocab);
-        const char* from = reinterpret_cast<const char*>(x + o.head);
+        const Span o = span_of(x, lo, hi);
+        const char* from = reinterpret_cast<const char*>(x + lo + o.head);
         const long long bytes = (long long)o.vecs * 16;
         for (int pass = 0; pass < loads; ++pass)
           for (long long at = 0; at < bytes; at += CHUNK) {
@@ -564,78 +751,59 @@ __global__ void __launch_bounds__(CTHREADS + 64, 2) distill_stream_kernel(const 
         mbar_wait_landed(&sm.full[st], phase);
       }
     }
-  } else if (warp == CWARPS + 1) {  // the entries
+    __syncwarp();
+  } else if (warp > CWARPS) {  // the entries
     pdl_wait();  // *norm
     Warp team;
-    long long it = 0;
-    long long before = -1;  // the row whose loss is still to be written
-    for (long long row = blockIdx.x;; row += grid, ++it) {
-      const int slot = it & 1;
-      if (row < a.rows) {
-        if (it >= 2) mbar_wait(&sm.freed[slot], ((it >> 1) - 1) & 1, &sm.failed);
-        StreamRow& h = sm.row[slot];
-        Entries e;
-        e.idx = reinterpret_cast<int*>(entry_mem + slot * per_slot);
-        e.p = reinterpret_cast<float*>(e.idx + a.k_pad);
-        e.x = e.p + a.k_pad;
-        e.hash = hash;
-        e.twice = &h.twice;
-        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-        if (MODE == DISTILL_GRAD) st = a.stats[row];
-        const Teacher t = prepare<T, MODE>(a, row, logits_row<T>(a, row), e, team, st);
-        if (lane == 0) {
-          h.t = t;
-          h.skip = t.w == 0.0f;
-          if (MODE == DISTILL_GRAD) h.m = st.m, h.s = st.s;
-          if (MODE != DISTILL_LOSS) h.G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);
-          mbar_arrive(&sm.told[slot]);
-        }
-        __syncwarp();
+    const int slot = warp - CWARPS - 1;
+    StreamRow& h = sm.row[slot];
+    const Entries e = entries_at(entry_mem + slot * per_slot, a, &h.twice);
+    uint32_t phase = 0;
+    for (long long row = row0 + slot * grid; row < a.rows; row += a.tellers * grid, phase ^= 1) {
+      if (row >= row0 + a.tellers * grid) mbar_wait(&sm.freed[slot], phase ^ 1, &sm.failed);
+      RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+      if (MODE == DISTILL_GRAD) st = a.stats[row];
+      const Teacher t = prepare<T, MODE>(a, row, logits_row<T>(a, row), e, team, st);
+      if (lane == 0) {
+        h.t = t;
+        h.skip = t.w == 0.0f;
+        if (MODE == DISTILL_GRAD) h.m = st.m, h.s = st.s;
+        if (MODE != DISTILL_LOSS) h.G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);
       }
-      if (MODE != DISTILL_GRAD && before >= 0) {  // the loss of the row before
-        const int was = slot ^ 1;
-        mbar_wait(&sm.stat[was], ((it - 1) >> 1) & 1, &sm.failed);
-        StreamRow& h = sm.row[was];
-        const Teacher t = h.t;
-        Entries e;
-        e.idx = reinterpret_cast<int*>(entry_mem + was * per_slot);
-        e.p = reinterpret_cast<float*>(e.idx + a.k_pad);
-        e.x = e.p + a.k_pad;
-        float loss = 0.0f;
-        if (t.live) {
-          const Expo ex(h.m, a.c);
-          loss = t.w * a.temperature * a.temperature * divergence(a, before, t, e, team, ex, h.s);
-        }
-        if (lane == 0) {
-          a.row_loss[before] = loss;
-          a.stats[before] = RowStats{h.m, h.s, t.tm, t.ts};
-        }
-        __syncwarp();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&sm.told[slot]);
+      if (MODE == DISTILL_GRAD) continue;
+      mbar_wait(&sm.stat[slot], phase, &sm.failed);
+      if (part != 0) continue;
+      float loss = 0.0f;
+      if (t.live) {
+        const Expo ex(h.m, a.c);
+        loss = t.w * a.temperature * a.temperature * divergence(a, t, e, team, ex, h.s);
       }
-      if (row >= a.rows) break;
-      before = row;
+      if (lane == 0) {
+        a.row_loss[row] = loss;
+        a.stats[row] = RowStats{h.m, h.s, t.tm, t.ts};
+      }
+      __syncwarp();
     }
   } else {
     const int tid = threadIdx.x;
     Consumers team(sm.red);
-    int st = 0;
-    uint32_t phase = 0;
-    long long it = 0;
-    for (long long row = blockIdx.x; row < a.rows; row += grid, ++it) {
-      const int slot = it & 1;
+    int st = 0, slot = 0;
+    uint32_t phase = 0, told = 0, joins = 0;
+    for (long long row = row0; row < a.rows; row += grid) {
       const T* x = logits_row<T>(a, row);
       T* g = MODE == DISTILL_LOSS ? nullptr : grad_row<T>(a, row);
-      const Span o = span_of(x, 0, a.vocab);
+      const Span o = span_of(x, lo, hi);
       const int chunks = (int)(((long long)o.vecs * 16 + CHUNK - 1) / CHUNK);
       const int at = edge_of<T>(o, tid);
       float edge = at >= 0 ? E::widen(x[at]) : -__int_as_float(0x7f800000);
-      uint4* gv = MODE == DISTILL_LOSS ? nullptr : reinterpret_cast<uint4*>(g + o.head);
-      mbar_wait(&sm.told[slot], (it >> 1) & 1, &sm.failed);
+      uint4* gv = MODE == DISTILL_LOSS ? nullptr : reinterpret_cast<uint4*>(g + lo + o.head);
+      mbar_wait(&sm.told[slot], told, &sm.failed);
       StreamRow& h = sm.row[slot];
-      const Teacher t = h.t;
-      const int skip = h.skip;
-      if (!t.live) {
-        if (!skip)  // weight, but no entry: the copies are under way
+      const bool live = h.t.live;
+      if (!live) {
+        if (!h.skip)  // weight, but no entry: the copies are under way
           for (int i = 0; i < chunks * loads; ++i) {
             mbar_wait(&sm.full[st], phase, &sm.failed);
             __syncwarp();
@@ -650,94 +818,97 @@ __global__ void __launch_bounds__(CTHREADS + 64, 2) distill_stream_kernel(const 
           h.m = 0.0f, h.s = 1.0f;
           mbar_arrive(&sm.stat[slot]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&sm.freed[slot]);
-        continue;
-      }
-      float m, s;
-      const int st0 = st;
-      if (MODE == DISTILL_GRAD) {
-        m = h.m, s = h.s;
       } else {
-        Running r{LOWEST, 0.0f};
-        for (int i = 0; i < chunks; ++i) {
-          mbar_wait(&sm.full[st], phase, &sm.failed);
-          const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)st * CHUNK);
-          const int n = o.vecs - i * (CHUNK / 16);
-          uint4 u[PER];
+        float m, s;
+        const int st0 = st;
+        if (MODE == DISTILL_GRAD) {
+          m = h.m, s = h.s;
+        } else {
+          Running r{LOWEST, 0.0f};
+          for (int i = 0; i < chunks; ++i) {
+            mbar_wait(&sm.full[st], phase, &sm.failed);
+            const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)st * CHUNK);
+            const int n = o.vecs - i * (CHUNK / 16);
+            uint4 u[PER];
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const int v = tid + j * CTHREADS;
-            u[j] = v < n ? buf[v] : E::none();
+            for (int j = 0; j < PER; ++j) {
+              const int v = tid + j * CTHREADS;
+              u[j] = v < n ? buf[v] : E::none();
+            }
+            if (MODE == DISTILL_LOSS || !a.resident) {
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&sm.empty[st]);
+            }
+            take<T, PER>(r, u, a.c);
+            if (++st == a.stages) st = 0, phase ^= 1;
           }
-          if (MODE == DISTILL_LOSS || !a.resident) {
+          take_one(r, edge, a.c);
+          r = team.joined(r, a.c);
+          if (parts > 1) {
+            // every part sends its statistics to all.  Two sets in turn: a part sends for row n + 2 after it has all of
+            // row n + 1, that is after every part has read row n's.
+            const int set = joins & 1;
+            if (tid == 0) mbar_expect(&sm.joined[set], parts * (uint32_t)sizeof(float2));
+            if (tid < parts) send_async(&sm.part[set][part], make_float2(r.m, r.s), &sm.joined[set], tid);
+            mbar_wait_cluster(&sm.joined[set], joins >> 1 & 1, &sm.failed);
+            ++joins;
+            r = Consumers::join_of(sm.part[set][lane % parts], parts, a.c);
+          }
+          m = r.m, s = r.s;
+          if (far_off(m, a.c)) {  // every part over the whole row: rare, and needs no exchange
+            s = far_sum(a, x, 0, a.vocab, m, team);
+            if (s == 0.0f) s = nan_f();  // every logit -inf: no distribution
+          }
+          if (tid == 0) {
+            h.m = m, h.s = s;
+            mbar_arrive(&sm.stat[slot]);
+          }
+        }
+        if (MODE != DISTILL_LOSS) {
+          const Expo ex(m, a.c);
+          const float G = h.G, gs = G / s;
+          int s2 = MODE == DISTILL_BOTH && a.resident ? st0 : st;
+          for (int i = 0; i < chunks; ++i) {
+            if (MODE == DISTILL_GRAD || !a.resident) mbar_wait(&sm.full[s2], phase, &sm.failed);
+            const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)s2 * CHUNK);
+            const int first = i * (CHUNK / 16), n = o.vecs - first;
+            uint4 u[PER];
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+              const int v = tid + j * CTHREADS;
+              if (v < n) u[j] = buf[v];
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sm.empty[st]);
-          }
-          take<T, PER>(r, u, a.c);
-          if (++st == a.stages) st = 0, phase ^= 1;
-        }
-        take_one(r, edge, a.c);
-        r = team.joined(r, a.c);
-        m = r.m, s = r.s;
-        if (far_off(m, a.c)) {
-          s = far_sum(a, x, 0, a.vocab, m, team);
-          if (s == 0.0f) s = nan_f();  // every logit -inf: no distribution
-        }
-        if (tid == 0) {
-          h.m = m, h.s = s;
-          mbar_arrive(&sm.stat[slot]);
-        }
-        __syncwarp();
-      }
-      if (MODE != DISTILL_LOSS) {
-        const Expo ex(m, a.c);
-        const float G = h.G, gs = G / s;
-        int s2 = MODE == DISTILL_BOTH && a.resident ? st0 : st;
-        for (int i = 0; i < chunks; ++i) {
-          if (MODE == DISTILL_GRAD || !a.resident) {
-            mbar_wait(&sm.full[s2], phase, &sm.failed);
-          }
-          const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)s2 * CHUNK);
-          const int first = i * (CHUNK / 16), n = o.vecs - first;
-          uint4 u[PER];
+            if (lane == 0) mbar_arrive(&sm.empty[s2]);
 #pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const int v = tid + j * CTHREADS;
-            if (v < n) u[j] = buf[v];
+            for (int j = 0; j < PER; ++j) {
+              const int v = tid + j * CTHREADS;
+              if (v < n) gv[first + v] = ex.scaled<T>(u[j], gs);
+            }
+            if (++s2 == a.stages) {
+              s2 = 0;
+              if (MODE == DISTILL_GRAD || !a.resident) phase ^= 1;
+            }
           }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&sm.empty[s2]);
-#pragma unroll
-          for (int j = 0; j < PER; ++j) {
-            const int v = tid + j * CTHREADS;
-            if (v < n) gv[first + v] = ex.scaled<T>(u[j], gs);
-          }
-          if (++s2 == a.stages) {
-            s2 = 0;
-            if (MODE == DISTILL_GRAD || !a.resident) phase ^= 1;
-          }
+          if (MODE == DISTILL_GRAD || !a.resident) st = s2;
+          if (at >= 0) g[at] = E::narrow(gs * ex(edge));
+          team.sync();
+          write_entries(a, g, entries_at(entry_mem + slot * per_slot, a, &h.twice), team, ex, gs, G, h.t.ts, lo, hi);
         }
-        if (MODE == DISTILL_GRAD || !a.resident) st = s2;
-        if (at >= 0) g[at] = E::narrow(gs * ex(edge));
-        team.sync();
-        Entries e;
-        e.idx = reinterpret_cast<int*>(entry_mem + slot * per_slot);
-        e.p = reinterpret_cast<float*>(e.idx + a.k_pad);
-        e.x = e.p + a.k_pad;
-        e.hash = nullptr;
-        e.twice = &h.twice;
-        write_entries(a, g, e, team, ex, gs, G, 0, a.vocab);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.freed[slot]);
+      if (++slot == a.tellers) slot = 0, told ^= 1;
     }
   }
-  __syncthreads();
+  if (parts > 1)
+    cluster.sync();  // nobody leaves while another part may still send to it
+  else
+    __syncthreads();
   if (sm.failed)  // a wait ran out (it never has): what this CTA wrote is not to be taken for a result
-    for (long long row = blockIdx.x + threadIdx.x * grid; row < a.rows; row += blockDim.x * grid) {
+    for (long long row = row0 + threadIdx.x * grid; row < a.rows; row += blockDim.x * grid) {
       if (MODE != DISTILL_GRAD) a.row_loss[row] = nan_f();
-      if (MODE != DISTILL_LOSS) grad_row<T>(a, row)[0] = E::narrow(nan_f());
+      if (MODE != DISTILL_LOSS && lo < hi) grad_row<T>(a, row)[lo] = E::narrow(nan_f());
     }
 }
 
@@ -812,7 +983,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
   }
   const Expo ex(st.m, a.c);
   if (MODE != DISTILL_GRAD && part == 0) {
-    const float d = divergence(a, row, t, e, team, ex, st.s);
+    const float d = divergence(a, t, e, team, ex, st.s);
     if (tid == 0) {
       a.row_loss[row] = t.w * a.temperature * a.temperature * d;
       a.stats[row] = RowStats{st.m, st.s, t.tm, t.ts};
@@ -830,7 +1001,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
     for (int i = tid; i < o.vecs; i += nthr) gv[i] = ex.scaled<T>(xv[i], gs);
   }
   __syncthreads();
-  write_entries(a, g, e, team, ex, gs, G, lo, hi);
+  write_entries(a, g, e, team, ex, gs, G, t.ts, lo, hi);
 }
 
 // One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double.
@@ -912,26 +1083,70 @@ static cudaError_t launch(K kernel, const DistillArgs& a, long long grid, int th
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
+// how many clusters of `parts` CTAs the GPU holds at a time (asked once per kernel, size and device)
+template <typename T, int MODE>
+static int most_clusters(int parts, int threads, size_t smem) {
+  const auto kernel = distill_stream_kernel<T, MODE>;
+  static std::atomic<int> known[64][4][MAX_TELLERS + 1];  // 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::atomic<int>& n = known[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3][(threads - CTHREADS - 32) / 32];
+  if (n.load() == 0) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * num_sms() / parts * parts), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = parts, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    int got = 0;
+    if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) got = 0;
+    n.store(got > 0 ? got : -1);
+  }
+  return n.load();
+}
+
 // `after`: the kernel before it in the stream is this call's sum of the weights
 template <typename T, int MODE>
 static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t stream) {
   constexpr int VE = Elem<T>::VE;
   const long long row_bytes = (long long)a.vocab * sizeof(T);
   const size_t entries = entry_bytes(a.k_pad, a.hash_size);
-  if (row_bytes <= 16 * SMALL_VECS * 32 && a.k <= 256)
-    return launch(distill_small_kernel<T, MODE, 32>, a, (a.rows + 3) / 4, 128, 4 * entries, 1, after, stream);
-  if (row_bytes <= 16 * SMALL_VECS * 128)
-    return launch(distill_small_kernel<T, MODE, 128>, a, a.rows, 128, entries, 1, after, stream);
   const int sms = num_sms();
-  if (a.rows >= sms) {
-    constexpr size_t LIMIT = 113 * 1024;  // two CTAs per SM
-    const size_t rest = (sizeof(StreamSmem) + 15) / 16 * 16 + entries + 12 * (size_t)a.k_pad;
-    a.stages = (int)((LIMIT - rest) / CHUNK);
+  constexpr size_t LIMIT = 113 * 1024;  // two CTAs per SM
+  if (row_bytes <= ROWS_MAX_BYTES && a.k <= 256) {
+    a.slot = (int)(row_bytes / 16 * 16);
+    int warps = ROWS_MAX_WARPS;
+    a.stages = ROWS_MAX_STAGES;
+    const auto bytes = [&] { return (size_t)warps * (a.stages * (size_t)a.slot + 4 * (size_t)a.hash_size); };
+    while (a.stages > 2 && bytes() > LIMIT) --a.stages;
+    while (bytes() > LIMIT) --warps;
+    long long grid = (a.rows + warps - 1) / warps;
+    if (grid > 2 * sms) grid = 2 * sms;
+    if (a.k <= 64) return launch(distill_rows_kernel<T, MODE, 2>, a, grid, warps * 32, bytes(), 1, after, stream);
+    return launch(distill_rows_kernel<T, MODE, 8>, a, grid, warps * 32, bytes(), 1, after, stream);
+  }
+  if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES) {
+    const size_t fixed = (sizeof(StreamSmem) + 15) / 16 * 16;
+    a.tellers = MAX_TELLERS;
+    while (a.tellers > 1 && a.tellers * entries > 24 * 1024) --a.tellers;
+    a.stages = (int)((LIMIT - fixed - a.tellers * entries) / CHUNK);
     if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
-    const long long chunks = (row_bytes + CHUNK - 1) / CHUNK;
-    a.resident = MODE == DISTILL_BOTH && chunks <= a.stages * 3 / 4;
-    const long long grid = a.rows < 2 * sms ? a.rows : 2 * sms;
-    return launch(distill_stream_kernel<T, MODE>, a, grid, CTHREADS + 64, a.stages * CHUNK + rest, 1, after, stream);
+    // with both passes in one call a row is to stay in the ring: large rows are shared by the CTAs of a cluster
+    const long long room = (long long)(a.stages * 3 / 4) * CHUNK;
+    int parts = 1;
+    if (MODE == DISTILL_BOTH)
+      while (parts < MAX_PARTS && row_bytes > parts * room) parts *= 2;
+    const size_t smem = a.stages * CHUNK + fixed + a.tellers * entries;
+    const int threads = CTHREADS + 32 + 32 * a.tellers;
+    const auto kernel = distill_stream_kernel<T, MODE>;
+    const int clusters = parts > 1 ? most_clusters<T, MODE>(parts, threads, smem) : 2 * sms;
+    if (clusters > 0) {
+      a.slice = ((a.vocab + parts - 1) / parts + 63) / 64 * 64;
+      a.resident = MODE == DISTILL_BOTH && row_bytes <= parts * room;
+      const long long grid = a.rows < clusters ? a.rows : clusters;
+      return launch(kernel, a, grid * parts, threads, smem, parts, after, stream);
+    }
   }
   // few rows: their columns are shared by clusters of up to 8 CTAs, so that all SMs have work
   int parts = 1;

@@ -15,6 +15,8 @@ struct Elem<float> {
   static constexpr int VE = 4;
   static __device__ __forceinline__ float widen(float v) { return v; }
   static __device__ __forceinline__ float narrow(float v) { return v; }
+  static __device__ __forceinline__ uint32_t raw(const float* p) { return *reinterpret_cast<const uint32_t*>(p); }
+  static __device__ __forceinline__ float of_raw(uint32_t w) { return __uint_as_float(w); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
   template <int N>
   static __device__ __forceinline__ float maximum(const uint4* u) {  // NaN is passed over, here and below
@@ -38,6 +40,8 @@ struct Elem<__nv_bfloat16> {
   static constexpr int VE = 8;
   static __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
   static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
+  static __device__ __forceinline__ uint32_t raw(const __nv_bfloat16* p) { return *reinterpret_cast<const unsigned short*>(p); }
+  static __device__ __forceinline__ float of_raw(uint32_t w) { return __uint_as_float(w << 16); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   template <int N>
   static __device__ __forceinline__ float maximum(const uint4* u) {
@@ -67,6 +71,8 @@ struct Elem<__half> {
   static constexpr int VE = 8;
   static __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
   static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
+  static __device__ __forceinline__ uint32_t raw(const __half* p) { return *reinterpret_cast<const unsigned short*>(p); }
+  static __device__ __forceinline__ float of_raw(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
   template <int N>
   static __device__ __forceinline__ float maximum(const uint4* u) {
@@ -134,6 +140,15 @@ __device__ __forceinline__ bool mbar_test(unsigned long long* b, uint32_t parity
       : "memory");
   return done;
 }
+__device__ __forceinline__ bool mbar_test_cluster(unsigned long long* b, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(done)
+      : "r"(smem_at(b)), "r"(parity)
+      : "memory");
+  return done;
+}
 constexpr int WAIT_LIMIT = 1 << 22;  // tries, each of which may sleep for a while: seconds, where a wait is microseconds
 // Waits for the phase; gives up when the limit is reached or another thread of the CTA has given up (*failed).  The
 // caller goes on in either case (its data are then worthless, its accesses in range) and the kernel ends as it should.
@@ -143,6 +158,21 @@ __device__ __forceinline__ void mbar_wait(unsigned long long* b, uint32_t parity
     if (mbar_test(b, parity) || *(volatile int*)failed) return;
   }
   *(volatile int*)failed = 1;
+}
+// the same for data that other CTAs of the cluster send
+__device__ __forceinline__ void mbar_wait_cluster(unsigned long long* b, uint32_t parity, int* failed) {
+  for (int i = 0; i < WAIT_LIMIT; ++i) {
+    if (mbar_test_cluster(b, parity) || *(volatile int*)failed) return;
+  }
+  *(volatile int*)failed = 1;
+}
+// 8 bytes to the address `to`, counted by the barrier `b`, of CTA `rank` of the cluster
+__device__ __forceinline__ void send_async(void* to, float2 v, unsigned long long* b, int rank) {
+  asm volatile(
+      "{\n .reg .b32 t, r;\n mapa.shared::cluster.u32 t, %0, %4;\n mapa.shared::cluster.u32 r, %3, %4;\n"
+      " st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [t], {%1, %2}, [r];\n}" ::"r"(smem_at(to)),
+      "f"(v.x), "f"(v.y), "r"(smem_at(b)), "r"(rank)
+      : "memory");
 }
 __device__ __forceinline__ void mbar_wait_landed(unsigned long long* b, uint32_t parity) {
   for (int i = 0; i < WAIT_LIMIT; ++i)

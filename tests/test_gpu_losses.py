@@ -1,4 +1,6 @@
 """The training losses on a B200 against 64-bit restatements (``loss_ref.py``), whose bounds count roundings."""
+import math
+
 import pytest
 import torch
 
@@ -105,29 +107,62 @@ def test_distillation_temperature_weights_reduction(dtype, temp, reduction):
     check_distill(x, t, idx, temp, None, reduction)
 
 
-def test_distillation_masks_and_absent_entries():
-    x, t, idx = distill_inputs(12, 1001, 8, "fp32", seed=5)
+# (copies of the twelve rows, columns): each kernel, the vocabulary within one CTA's columns and shared by a cluster
+REGIMES = [(1, 1001), (150, 1001), (1, 4095), (1, 20011), (13, 9003), (26, 30001), (13, 70003)]
+
+
+@pytest.mark.parametrize("copies, vocab", REGIMES)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("k", [8, 90, 300])
+def test_distillation_masks_and_absent_entries(copies, vocab, dtype, k):
+    x, t, idx = distill_inputs(12, vocab, k, dtype, seed=5)
+    low = torch.finfo(DT[dtype]).min
     idx[0, 3:] = -1          # a shorter list
     idx[1] = -1              # none at all
     t[2] = -INF              # none at all
     t[3, 1:] = -INF          # one
     idx[4, 1] = idx[4, 0]    # the same index twice
-    idx[5] = idx[5, 0]       # eight times
-    x[6, 500:] = -INF        # columns that the student may not use ...
-    idx[6] = torch.arange(8, device=device())
-    x[7, :] = torch.finfo(torch.float32).min
+    idx[5] = idx[5, 0]       # many times
+    idx[6] = torch.arange(k, device=device())
+    x[6, k + vocab // 2:] = -INF  # columns that the student may not use ...
+    x[7, :] = low
     x[7, 17] = 0.0
     idx[7, 0] = 17
     t[7, 1:] = -INF
-    x[8, :] = torch.finfo(torch.float32).min  # all of the lowest value: uniform
+    x[8, :] = low            # all of the lowest value: uniform
     x[9, idx[9, 0]] = -INF   # ... an entry among them: infinite loss
     x[10], idx[10, 0] = float("nan"), 5
     w = torch.ones(12, device=device())
     w[10] = 0                # a padded row may hold anything
     w[11] = -2.0
-    for reduction in ("none", "sum"):
-        check_distill(x, t, idx, 1.0, w, reduction)
-    check_distill(x, t, idx, 2.0, w, "none")
+    for temp, reduction in ((1.0, "none"), (1.0, "sum"), (2.0, "none")):
+        check_distill_copies(copies, x, t, idx, temp, w, reduction)
+
+
+def check_distill_copies(copies, x, t, idx, temp, w, reduction):
+    """Twelve different rows, so many times that another kernel takes them.  Every copy keeps the bounds; copies that lie alike to
+    the 16-byte boundaries, by which a row is cut into vectors and so its sums into parts, have the same bits."""
+    if copies == 1:
+        check_distill(x, t, idx, temp, w, reduction)
+        return
+    f, n = F(), x.shape[0]
+    loss, q, p = distill_ref(x, t, idx, temp, w)
+    rb = torch.tensor([distill_row_bound(x.shape[1], temp, float(a)) for a in w], dtype=torch.float64)
+    coef = (w.double().cpu() * temp).view(-1, 1)
+    gref = coef * (q - p)
+    gb = distill_grad_bound(gref, coef.abs() * q, coef.abs() * p, 1.0, x.shape[1], x.dtype)
+    many = [v.repeat(copies, *[1] * (v.dim() - 1)) for v in (x, t, idx, w)]
+    got, grad = f.topk_distillation_with_grad(*many[:3], temp, many[3], "none")
+    leaf = many[0].requires_grad_()
+    out = f.topk_distillation(leaf, *many[1:3], temp, many[3], reduction)
+    (auto,) = torch.autograd.grad(out.sum(), leaf)
+    rows = out if reduction == "none" else f.topk_distillation(leaf.detach(), *many[1:3], temp, many[3], "none")
+    for v, ref, bound in ((got, loss, rb), (rows, loss, rb), (grad, gref, gb), (auto, gref, gb)):
+        v = v.detach().view(copies, n, -1)
+        alike = 16 // math.gcd(16, n * x.shape[1] * x.element_size())
+        assert all(same_bits(v[0], v[c]) for c in range(alike, copies, alike)), "copies of a row differ"
+        for c in range(min(alike, copies)):
+            close(v[c], ref.view(n, -1), bound.view(n, -1))
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
