@@ -95,7 +95,7 @@ __device__ __forceinline__ void take(Running& r, const uint4* u, float c) {
   r.s *= ex2(ref_of(r.m, c) - ref);
   r.m = m;
   const f2 c2 = f2_splat(c), ref2 = f2_splat(-ref);
-  f2 sum = f2_splat(0.0f);
+  f2 sum[2] = {f2_splat(0.0f), f2_splat(0.0f)};
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     float x[E::VE];
@@ -104,11 +104,11 @@ __device__ __forceinline__ void take(Running& r, const uint4* u, float c) {
     for (int i = 0; i < E::VE; i += 2) {
       float a, b;
       f2_unpack(f2_fma(f2_pack(x[i], x[i + 1]), c2, ref2), a, b);
-      sum = f2_add(sum, f2_pack(ex2(a), ex2(b)));
+      sum[i / 2 % 2] = f2_add(sum[i / 2 % 2], f2_pack(ex2(a), ex2(b)));
     }
   }
   float a, b;
-  f2_unpack(sum, a, b);
+  f2_unpack(f2_add(sum[0], sum[1]), a, b);
   r.s += a + b;
 }
 
@@ -146,13 +146,19 @@ struct Expo {
   }
 };
 
+// first element of a row; rows < 2^28, so the division is one of 32 bits
+__device__ __forceinline__ long long row_at(long long row, long long inner, long long outer_stride, long long inner_stride) {
+  if (inner == 1) return row * outer_stride;
+  const unsigned o = (unsigned)row / (unsigned)inner;
+  return o * outer_stride + ((unsigned)row - o * (unsigned)inner) * inner_stride;
+}
 template <typename T>
 __device__ __forceinline__ const T* logits_row(const DistillArgs& a, long long row) {
-  return reinterpret_cast<const T*>(a.logits) + (row / a.inner) * a.outer_stride + (row % a.inner) * a.inner_stride;
+  return reinterpret_cast<const T*>(a.logits) + row_at(row, a.inner, a.outer_stride, a.inner_stride);
 }
 template <typename T>
 __device__ __forceinline__ T* grad_row(const DistillArgs& a, long long row) {
-  return reinterpret_cast<T*>(a.grad) + (row / a.inner) * a.grad_outer_stride + (row % a.inner) * a.grad_inner_stride;
+  return reinterpret_cast<T*>(a.grad) + row_at(row, a.inner, a.grad_outer_stride, a.grad_inner_stride);
 }
 
 // Columns [lo, hi) of a row in steps of 16 bytes: up to VE - 1 single columns before the first boundary, vectors, the
@@ -282,7 +288,7 @@ __device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, 
   t.tm = LOWEST;
   bool any = false, bad = false;
   if (team.rank() == 0) *e.twice = 0;
-#pragma unroll 2
+#pragma unroll 4
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const long long i = load_index(a.index, row * a.k + k, a.index_bits);
     const float v = load_any(a.teacher, row * a.k + k, a.teacher_dtype);
@@ -335,7 +341,7 @@ __device__ __forceinline__ float divergence(const DistillArgs& a, const Teacher&
     if (e.idx[k] < 0 || p == 0.0f) continue;
     sum += p * (z - ex.log2_of(e.x[k]));
   }
-  return LN2 * (team.sum(sum) / t.ts) + (logf(s) - logf(t.ts));
+  return LN2 * (team.sum(sum) * rcp_nr(t.ts) + (lg2(s) - lg2(t.ts)));
 }
 
 // The entries' columns within [lo, hi): q - p, written over q.  After a barrier behind the stores of q.
@@ -343,7 +349,7 @@ template <typename T, typename Team>
 __device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const Entries& e, const Team& team,
                                               const Expo& ex, float gs, float G, float ts, int lo, int hi) {
   const bool twice = *e.twice;
-  const float Gp = G / ts;
+  const float Gp = G * rcp_nr(ts);
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const int i = e.idx[k];
     if (i < lo || i >= hi) continue;
@@ -357,6 +363,16 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const 
     }
     g[i] = Elem<T>::narrow(gs * ex(e.x[k]) - Gp * p);
   }
+}
+
+// brings a row's entries into L2
+__device__ __forceinline__ void prefetch_entries(const DistillArgs& a, long long row) {
+  const char* i = reinterpret_cast<const char*>(a.index) + row * a.k * (a.index_bits / 8);
+  const int ni = a.k * (a.index_bits / 8), size = a.teacher_dtype == LPMM_B200_DTYPE_FP32 ? 4 : 2;
+  const char* t = reinterpret_cast<const char*>(a.teacher) + row * a.k * size;
+  const int lane = threadIdx.x & 31;
+  for (int at = lane * 128; at < ni; at += 32 * 128) prefetch_l2(i + at);
+  for (int at = lane * 128; at < a.k * size; at += 32 * 128) prefetch_l2(t + at);
 }
 
 __device__ __forceinline__ float upstream_of(const DistillArgs& a, long long row) {
@@ -424,152 +440,159 @@ struct RowFetch {
 };
 
 template <typename T, int MODE, int KV>
-__global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, 2) distill_rows_kernel(const DistillArgs a) {
+__global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_rows_kernel(const DistillArgs a) {
   using E = Elem<T>;
   extern __shared__ __align__(16) char smem[];
   __shared__ unsigned long long full[ROWS_MAX_WARPS][ROWS_MAX_STAGES];
   __shared__ int failed;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  char* slots = smem + (size_t)warp * a.stages * a.slot;
-  int* hash = reinterpret_cast<int*>(smem + (size_t)warps * a.stages * a.slot) + warp * a.hash_size;
+  char* slots = smem + warp * a.stages * a.slot;
   if (lane == 0) {
     for (int i = 0; i < a.stages; ++i) mbar_init(&full[warp][i], 1);
     mbar_fence();
   }
   if (threadIdx.x == 0) failed = 0;
-  if (MODE != DISTILL_LOSS)
-    for (int i = lane; i < a.hash_size; i += 32) hash[i] = -1;
   __syncthreads();
-  const long long stride = (long long)gridDim.x * warps, row0 = (long long)blockIdx.x * warps + warp;
+  const int rows = (int)a.rows, stride = gridDim.x * warps, row0 = blockIdx.x * warps + warp;
   // bit i of `dead`: row number 32 n + i of this warp has weight 0 and is not copied; `dead_next`: of the next 32
-  auto weights_of = [&](long long it) {
-    const long long r = row0 + (it + lane) * stride;
-    return __ballot_sync(~0u, a.weights && r < a.rows && a.weights[r] == 0.0f);
+  auto weights_of = [&](int it) {
+    const long long r = row0 + (long long)(it + lane) * stride;
+    return __ballot_sync(~0u, a.weights && r < rows && a.weights[r] == 0.0f);
   };
   uint32_t dead = weights_of(0), dead_next = weights_of(32);
-  auto copy = [&](long long it, int st, bool none) {
-    const long long row = row0 + it * stride;
-    if (lane != 0 || row >= a.rows) return;
+  auto copy = [&](long long row, int st, bool none) {
+    if (lane != 0 || row >= rows) return;
     const T* x = logits_row<T>(a, row);
     const Span o = span_of(x, 0, a.vocab);
     const uint32_t n = none ? 0 : o.vecs * 16;
     mbar_expect(&full[warp][st], n);
-    if (n) bulk_load(slots + (size_t)st * a.slot, x + o.head, n, &full[warp][st]);
+    if (n) bulk_load(slots + st * a.slot, x + o.head, n, &full[warp][st]);
   };
-  for (int i = 0; i < a.stages; ++i) copy(i, i, dead >> i & 1);
+  for (int i = 0; i < a.stages; ++i) copy(row0 + (long long)i * stride, i, dead >> i & 1);
   RowFetch<T, MODE, KV> next;
   next.load(a, row0);
   pdl_wait();
-  const float up0 = a.scale * (a.norm ? *a.norm : 1.0f);
-  int st = 0;
+  const float up0 = a.scale * a.temperature * (a.norm ? *a.norm : 1.0f);
+  int st = 0, it = 0;
   uint32_t phase = 0;
-  for (long long it = 0, row = row0; row < a.rows; ++it, row += stride) {
-    RowFetch<T, MODE, KV> f = next;
+  for (long long row = row0; row < rows; ++it, row += stride) {
+    const RowFetch<T, MODE, KV> f = next;
     next.load(a, row + stride);
     const T* x = logits_row<T>(a, row);
     const Span o = span_of(x, 0, a.vocab);
-    const T* xs = reinterpret_cast<const T*>(slots + (size_t)st * a.slot);  // column head is its first
-    const uint4* buf = reinterpret_cast<const uint4*>(xs);
+    const bool edges = o.head + o.tail != 0;
+    char* slot = slots + st * a.slot;
+    const T* xs = reinterpret_cast<const T*>(slot);  // column `head` is its first
+    const uint4* buf = reinterpret_cast<const uint4*>(slot);
     mbar_wait(&full[warp][st], phase, &failed);
 
     // entries
     int idx[KV];
-    float tk[KV], tm = LOWEST;
-    const float edge = f.edge();
+    float z[KV], xk[KV], tm = LOWEST;
     bool any = false, bad = false;
 #pragma unroll
     for (int j = 0; j < KV; ++j) {
       const long long i = f.index(a, j);
-      tk[j] = f.teacher(a, j);
-      const bool entry = i >= 0 && tk[j] != -__int_as_float(0x7f800000);
+      z[j] = f.teacher(a, j);
+      const bool entry = i >= 0 && z[j] != -__int_as_float(0x7f800000);
       const bool in = entry && i < a.vocab;  // an index outside of the vocabulary is not followed
       bad |= entry && !in;
       any |= entry;
       idx[j] = in ? (int)i : -1;
-      if (entry) tm = fmaxf(tm, tk[j]);
+      if (entry) tm = fmaxf(tm, z[j]);
     }
     const bool live = __any_sync(~0u, any) && f.w != 0.0f;
-    bad = __any_sync(~0u, bad);
-    float xk[KV];
+    if (live) {
 #pragma unroll
-    for (int j = 0; j < KV; ++j) {
-      const int i = idx[j];
-      xk[j] = 0.0f;
-      if (i >= 0 && live) xk[j] = E::widen(i >= o.head && i < o.tail_at ? xs[i - o.head] : x[i]);
-    }
-
-    // statistics
-    Running r{LOWEST, 0.0f};
-    float ts = 0.0f;
-    if (MODE != DISTILL_GRAD && live) {
-      for (int v = lane; v < o.vecs; v += 128) {
-        uint4 u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = v + 32 * j < o.vecs ? buf[v + 32 * j] : E::none();
-        take<T, 4>(r, u, a.c);
+      for (int j = 0; j < KV; ++j) {
+        const int i = idx[j];
+        xk[j] = 0.0f;
+        if (i >= 0) xk[j] = E::widen(i >= o.head && i < o.tail_at ? xs[i - o.head] : x[i]);
       }
-      take_one(r, edge, a.c);
-      float m = r.m;
+      // statistics
+      Running r{LOWEST, 0.0f};
+      float ts = 0.0f, p[KV];
+      if (MODE == DISTILL_GRAD) {
+        tm = f.st.tm, ts = f.st.ts, r.m = f.st.m, r.s = f.st.s;
+      } else {
+        for (int v = lane; v < o.vecs; v += 128) {
+          uint4 u[4];
 #pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-        tm = fmaxf(tm, __shfl_xor_sync(~0u, tm, d));
-      }
-      r.s *= ex2(ref_of(r.m, a.c) - ref_of(m, a.c));
-      r.m = m;
-    }
-    if (MODE == DISTILL_GRAD) tm = f.st.tm, ts = f.st.ts, r.m = f.st.m, r.s = f.st.s;
-    float z[KV], p[KV];
+          for (int j = 0; j < 4; ++j) u[j] = v + 32 * j < o.vecs ? buf[v + 32 * j] : E::none();
+          take<T, 4>(r, u, a.c);
+        }
+        if (edges) take_one(r, f.edge(), a.c);
+        float m = r.m;
 #pragma unroll
-    for (int j = 0; j < KV; ++j) {
-      z[j] = (tk[j] - tm) * a.c;
-      p[j] = idx[j] >= 0 ? ex2(z[j]) : 0.0f;
-      if (MODE != DISTILL_GRAD) ts += p[j];
-    }
-    if (MODE != DISTILL_GRAD && live) {
+        for (int d = 16; d; d >>= 1) {
+          m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
+          tm = fmaxf(tm, __shfl_xor_sync(~0u, tm, d));
+        }
+        r.s *= ex2(ref_of(r.m, a.c) - ref_of(m, a.c));
+        r.m = m;
+      }
 #pragma unroll
-      for (int d = 16; d; d >>= 1) {
-        r.s += __shfl_xor_sync(~0u, r.s, d);
-        ts += __shfl_xor_sync(~0u, ts, d);
+      for (int j = 0; j < KV; ++j) {
+        z[j] = (z[j] - tm) * a.c;
+        p[j] = idx[j] >= 0 ? ex2(z[j]) : 0.0f;
+        if (MODE != DISTILL_GRAD) ts += p[j];
       }
-      if (bad) ts = nan_f();
-      if (far_off(r.m, a.c)) {
-        Warp team;
-        r.s = far_sum(a, x, 0, a.vocab, r.m, team);
-        if (r.s == 0.0f) r.s = nan_f();  // every logit -inf: no distribution
-      }
-    }
-    const Expo ex(r.m, a.c);
-    if (MODE != DISTILL_GRAD) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int j = 0; j < KV; ++j)
-        if (p[j] != 0.0f) sum += p[j] * (z[j] - ex.log2_of(xk[j]));
-      sum = Warp().sum(sum);
-      if (lane == 0) {
-        a.row_loss[row] = live ? f.w * a.temperature * a.temperature * (LN2 * (sum / ts) + (logf(r.s) - logf(ts))) : 0.0f;
-        a.stats[row] = RowStats{r.m, r.s, tm, ts};
-      }
-    }
-    if (MODE != DISTILL_LOSS) {
-      T* g = grad_row<T>(a, row);
-      uint4* gv = reinterpret_cast<uint4*>(g + o.head);
-      const int at = edge_of<T>(o, lane);
-      const float G = live ? up0 * (MODE == DISTILL_GRAD ? f.up : 1.0f) * f.w * a.temperature + (ts - ts) : 0.0f;
-      const float gs = G / r.s, Gp = G / ts;
-      if (live) {
-        for (int v = lane; v < o.vecs; v += 32) gv[v] = ex.scaled<T>(buf[v], gs);
-        if (at >= 0) g[at] = E::narrow(gs * ex(edge));
-        bool twice = false;
+      const Expo ex(r.m, a.c);
+      if (MODE != DISTILL_GRAD) {
+        float sum = 0.0f;
 #pragma unroll
         for (int j = 0; j < KV; ++j)
-          if (idx[j] >= 0) twice |= seen(hash, a.hash_size, idx[j]);
-        __syncwarp();
-        for (int i = lane; i < a.hash_size; i += 32) hash[i] = -1;
-        bool mine[KV];
+          if (p[j] != 0.0f) sum += p[j] * (z[j] - ex.log2_of(xk[j]));
 #pragma unroll
-        for (int j = 0; j < KV; ++j) mine[j] = idx[j] >= 0;
-        if (__any_sync(~0u, twice)) {  // an index that occurs several times: its first entry writes for all, in their order
+        for (int d = 16; d; d >>= 1) {
+          r.s += __shfl_xor_sync(~0u, r.s, d);
+          ts += __shfl_xor_sync(~0u, ts, d);
+          sum += __shfl_xor_sync(~0u, sum, d);
+        }
+        if (__any_sync(~0u, bad)) ts = nan_f();
+        if (ex.far) {
+          Warp team;
+          r.s = far_sum(a, x, 0, a.vocab, r.m, team);
+          if (r.s == 0.0f) r.s = nan_f();  // every logit -inf: no distribution
+        }
+        if (lane == 0) {
+          a.row_loss[row] = f.w * a.temperature * a.temperature * LN2 * (sum * rcp_nr(ts) + (lg2(r.s) - lg2(ts)));
+          a.stats[row] = RowStats{r.m, r.s, tm, ts};
+        }
+      }
+      if (MODE != DISTILL_LOSS) {
+        T* g = grad_row<T>(a, row);
+        uint4* gv = reinterpret_cast<uint4*>(g + o.head);
+        const float G = up0 * (MODE == DISTILL_GRAD ? f.up : 1.0f) * f.w + (ts - ts);
+        const float gs = G * rcp_nr(r.s), Gp = G * rcp_nr(ts);
+        for (int v = lane; v < o.vecs; v += 128) {
+          uint4 u[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (v + 32 * j < o.vecs) u[j] = buf[v + 32 * j];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (v + 32 * j < o.vecs) gv[v + 32 * j] = ex.scaled<T>(u[j], gs);
+        }
+        if (edges) {
+          const int at = edge_of<T>(o, lane);
+          if (at >= 0) g[at] = E::narrow(gs * ex(f.edge()));
+        }
+        // the row is not needed any more: its slot shows an index that occurs twice, by the second one's number
+        unsigned short* claim = reinterpret_cast<unsigned short*>(slot);
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < KV; ++j)
+          if (idx[j] >= 0) claim[idx[j]] = (unsigned short)(lane + 32 * j);
+        __syncwarp();
+        bool mine[KV], twice = false;
+#pragma unroll
+        for (int j = 0; j < KV; ++j) {
+          mine[j] = idx[j] >= 0;
+          twice |= mine[j] && claim[idx[j]] != lane + 32 * j;
+        }
+        bulk_load_fence();
+        if (__any_sync(~0u, twice)) {  // its first entry writes for all, in their order
           float all[KV];
 #pragma unroll
           for (int j = 0; j < KV; ++j) all[j] = 0.0f;
@@ -591,8 +614,17 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, 2) distill_rows_kernel(co
 #pragma unroll
         for (int j = 0; j < KV; ++j)
           if (mine[j]) g[idx[j]] = E::narrow(gs * ex(xk[j]) - Gp * p[j]);
-      } else {
+      }
+    } else {
+      if (MODE != DISTILL_GRAD && lane == 0) {
+        a.row_loss[row] = 0.0f;
+        a.stats[row] = RowStats{0.0f, 1.0f, 0.0f, 0.0f};
+      }
+      if (MODE != DISTILL_LOSS) {
+        T* g = grad_row<T>(a, row);
+        uint4* gv = reinterpret_cast<uint4*>(g + o.head);
         for (int v = lane; v < o.vecs; v += 32) gv[v] = make_uint4(0, 0, 0, 0);
+        const int at = edge_of<T>(o, lane);
         if (at >= 0) g[at] = E::narrow(0.0f);
       }
     }
@@ -601,14 +633,14 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, 2) distill_rows_kernel(co
       dead = dead_next;
       dead_next = weights_of(it + 33);
     }
-    // row number it + stages takes the slot; its bit is in the current word (which from here on is that of it + 1) or the next
-    const int ahead = (int)((it + 1) & 31) + a.stages - 1;
-    copy(it + a.stages, st, (ahead < 32 ? dead >> ahead : dead_next >> (ahead - 32)) & 1);
+    // row number it + stages takes the slot; its bit is in the word of row number it + 1 or in the next one
+    const int ahead = ((it + 1) & 31) + a.stages - 1;
+    copy(row + (long long)a.stages * stride, st, (ahead < 32 ? dead >> ahead : dead_next >> (ahead - 32)) & 1);
     if (++st == a.stages) st = 0, phase ^= 1;
   }
   __syncthreads();
   if (failed)  // a wait ran out (it never has): what this CTA wrote is not to be taken for a result
-    for (long long row = row0; row < a.rows; row += stride)
+    for (long long row = row0; row < rows; row += stride)
       if (lane == 0) {
         if (MODE != DISTILL_GRAD) a.row_loss[row] = nan_f();
         if (MODE != DISTILL_LOSS) grad_row<T>(a, row)[0] = E::narrow(nan_f());
@@ -619,10 +651,19 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, 2) distill_rows_kernel(co
 // stream: persistent CTAs, or clusters of them that share the columns of a row; one warp copies the rows into a ring of
 // chunks, a few prepare the entries of the next rows, eight take the passes
 // ---------------------------------------------------------------------------------------------
-constexpr int CHUNK = 8192;
-constexpr int CWARPS = 8, CTHREADS = CWARPS * 32;
-constexpr int PER = CHUNK / 16 / CTHREADS;  // vectors per thread and chunk
+constexpr int PER = 4;  // vectors per consuming thread and chunk
 constexpr int MAX_STAGES = 14, MAX_TELLERS = 4, MAX_PARTS = 8;
+
+// CW: consuming warps.  Eight with chunks of 16 KB in two CTAs per SM, or four with chunks of 8 KB in four or five: more
+// rows under way at a time hide what a row costs beside its columns (a reduction, a barrier or two), but leave each less
+// room to stay in the ring.
+template <int MODE, int CW>
+struct Shape {
+  static constexpr int CHUNK = 2048 * CW, THREADS = 32 * CW;
+  static constexpr int CTAS = CW == 8 ? 2 : MODE == DISTILL_BOTH ? 4 : 5;
+  static constexpr int TELLERS = CW == 8 ? 4 : MODE == DISTILL_BOTH ? 2 : 1;
+  static constexpr size_t ROOM = 227 * 1024 / CTAS - 1024;
+};
 
 struct StreamRow {  // what the consumers are told about a row, and what they tell
   Teacher t;
@@ -633,22 +674,23 @@ struct StreamRow {  // what the consumers are told about a row, and what they te
 struct StreamSmem {
   unsigned long long full[MAX_STAGES], empty[MAX_STAGES];
   // per slot: entries ready / no longer read / statistics of the row known
-  unsigned long long told[MAX_TELLERS], freed[MAX_TELLERS], stat[MAX_TELLERS];
+  unsigned long long told[2 * MAX_TELLERS], freed[2 * MAX_TELLERS], stat[2 * MAX_TELLERS];
   unsigned long long joined[2];  // the statistics of all parts of a row are in `part`
   float2 part[2][MAX_PARTS];
-  StreamRow row[MAX_TELLERS];
-  float2 red[2][CWARPS];
+  StreamRow row[2 * MAX_TELLERS];
+  float2 red[2][8];
   int failed;
 };
 
 // the consumers as a team: named barrier 1
+template <int CW>
 struct Consumers {
-  float2 (*red)[CWARPS];
+  float2 (*red)[8];
   int turn = 0;
-  __device__ __forceinline__ explicit Consumers(float2 (*r)[CWARPS]) : red(r) {}
+  __device__ __forceinline__ explicit Consumers(float2 (*r)[8]) : red(r) {}
   __device__ __forceinline__ int rank() const { return threadIdx.x; }
-  __device__ __forceinline__ int size() const { return CTHREADS; }
-  __device__ __forceinline__ void sync() const { asm volatile("bar.sync 1, %0;" ::"n"(CTHREADS) : "memory"); }
+  __device__ __forceinline__ int size() const { return CW * 32; }
+  __device__ __forceinline__ void sync() const { asm volatile("bar.sync 1, %0;" ::"n"(CW * 32) : "memory"); }
   __device__ __forceinline__ float2* exchange(float2 v) {
     float2* r = red[turn ^= 1];
     if ((threadIdx.x & 31) == 0) r[threadIdx.x >> 5] = v;
@@ -658,7 +700,7 @@ struct Consumers {
   __device__ __forceinline__ float sum(float v) {
     const float2* r = exchange(make_float2(Warp().sum(v), 0.0f));
     v = r[0].x;
-    for (int i = 1; i < CWARPS; ++i) v += r[i].x;
+    for (int i = 1; i < CW; ++i) v += r[i].x;
     return v;
   }
   // of n <= 8 values that lanes 0 ... n - 1, repeated over the warp, hold
@@ -675,18 +717,21 @@ struct Consumers {
   }
   __device__ __forceinline__ Running joined(Running v, float c) {
     v = warp_join(v, c);
-    return join_of(exchange(make_float2(v.m, v.s))[threadIdx.x % CWARPS], CWARPS, c);
+    return join_of(exchange(make_float2(v.m, v.s))[threadIdx.x % CW], CW, c);
   }
 };
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_stream_kernel(const DistillArgs a) {
+template <typename T, int MODE, int CW>
+__global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shape<MODE, CW>::CTAS)
+    distill_stream_kernel(const DistillArgs a) {
   using E = Elem<T>;
+  constexpr int CHUNK = Shape<MODE, CW>::CHUNK, CTHREADS = Shape<MODE, CW>::THREADS;
   extern __shared__ __align__(16) char smem[];
   char* ring = smem;
   StreamSmem& sm = *reinterpret_cast<StreamSmem*>(smem + (size_t)a.stages * CHUNK);
   char* entry_mem = smem + (size_t)a.stages * CHUNK + (sizeof(StreamSmem) + 15) / 16 * 16;
-  const size_t per_slot = entry_bytes(a.k_pad, a.hash_size);
+  const size_t per_slot = entry_bytes(a.k_pad, 0);
+  int* hashes = reinterpret_cast<int*>(entry_mem + 2 * a.tellers * per_slot);
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int lo = min(part * a.slice, a.vocab), hi = min(lo + a.slice, a.vocab);
@@ -694,21 +739,18 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
       mbar_init(&sm.full[i], 1);
-      mbar_init(&sm.empty[i], CWARPS);
+      mbar_init(&sm.empty[i], CW);
     }
-    for (int i = 0; i < a.tellers; ++i) {
+    for (int i = 0; i < 2 * a.tellers; ++i) {
       mbar_init(&sm.told[i], 1);
-      mbar_init(&sm.freed[i], CWARPS);
+      mbar_init(&sm.freed[i], CW);
       mbar_init(&sm.stat[i], 1);
     }
     for (int i = 0; i < 2; ++i) mbar_init(&sm.joined[i], 1);
     sm.failed = 0;
     mbar_fence();
   }
-  for (int j = 0; j < a.tellers; ++j) {
-    int* hash = entries_at(entry_mem + j * per_slot, a, nullptr).hash;
-    for (int i = threadIdx.x; i < a.hash_size; i += blockDim.x) hash[i] = -1;
-  }
+  for (int i = threadIdx.x; i < a.tellers * a.hash_size; i += blockDim.x) hashes[i] = -1;
   if (parts > 1)
     cluster.sync();
   else
@@ -717,7 +759,7 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
   // passes over the chunks: once where the row stays in the ring, or only one pass is made
   const int loads = MODE == DISTILL_BOTH && !a.resident ? 2 : 1;
 
-  if (warp == CWARPS) {  // the copies
+  if (warp == CW) {  // the copies
     int st = 0, fills = 0;
     uint32_t phase = 0, skips = 0;
     long long it = 0;
@@ -752,43 +794,56 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
       }
     }
     __syncwarp();
-  } else if (warp > CWARPS) {  // the entries
+  } else if (warp > CW) {  // the entries
     pdl_wait();  // *norm
     Warp team;
-    const int slot = warp - CWARPS - 1;
-    StreamRow& h = sm.row[slot];
-    const Entries e = entries_at(entry_mem + slot * per_slot, a, &h.twice);
-    uint32_t phase = 0;
-    for (long long row = row0 + slot * grid; row < a.rows; row += a.tellers * grid, phase ^= 1) {
-      if (row >= row0 + a.tellers * grid) mbar_wait(&sm.freed[slot], phase ^ 1, &sm.failed);
-      RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
-      if (MODE == DISTILL_GRAD) st = a.stats[row];
-      const Teacher t = prepare<T, MODE>(a, row, logits_row<T>(a, row), e, team, st);
-      if (lane == 0) {
-        h.t = t;
-        h.skip = t.w == 0.0f;
-        if (MODE == DISTILL_GRAD) h.m = st.m, h.s = st.s;
-        if (MODE != DISTILL_LOSS) h.G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);
+    const int teller = warp - CW - 1;
+    const long long step = a.tellers * grid;
+    long long before = -1;  // the row whose loss is still to be written
+    int n = 0;              // rows begun; row number n has slot teller + (n & 1) * tellers
+    for (long long row = row0 + teller * grid;; row += step, ++n) {
+      if (row < a.rows) {
+        const int slot = teller + (n & 1) * a.tellers;
+        StreamRow& h = sm.row[slot];
+        Entries e = entries_at(entry_mem + slot * per_slot, a, &h.twice);
+        e.hash = hashes + teller * a.hash_size;
+        if (n >= 2) mbar_wait(&sm.freed[slot], (n >> 1 & 1) ^ 1, &sm.failed);
+        RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
+        if (MODE == DISTILL_GRAD) st = a.stats[row];
+        const Teacher t = prepare<T, MODE>(a, row, logits_row<T>(a, row), e, team, st);
+        if (lane == 0) {
+          h.t = t;
+          h.skip = t.w == 0.0f;
+          if (MODE == DISTILL_GRAD) h.m = st.m, h.s = st.s;
+          if (MODE != DISTILL_LOSS) h.G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.told[slot]);
+        if (row + step < a.rows) prefetch_entries(a, row + step);
       }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&sm.told[slot]);
-      if (MODE == DISTILL_GRAD) continue;
-      mbar_wait(&sm.stat[slot], phase, &sm.failed);
-      if (part != 0) continue;
-      float loss = 0.0f;
-      if (t.live) {
-        const Expo ex(h.m, a.c);
-        loss = t.w * a.temperature * a.temperature * divergence(a, t, e, team, ex, h.s);
+      if (MODE != DISTILL_GRAD && before >= 0) {
+        const int slot = teller + ((n - 1) & 1) * a.tellers;
+        const StreamRow& h = sm.row[slot];
+        mbar_wait(&sm.stat[slot], (n - 1) >> 1 & 1, &sm.failed);
+        if (part == 0) {
+          const Teacher t = h.t;
+          float loss = 0.0f;
+          if (t.live)
+            loss = t.w * a.temperature * a.temperature *
+                   divergence(a, t, entries_at(entry_mem + slot * per_slot, a, nullptr), team, Expo(h.m, a.c), h.s);
+          if (lane == 0) {
+            a.row_loss[before] = loss;
+            a.stats[before] = RowStats{h.m, h.s, t.tm, t.ts};
+          }
+        }
+        __syncwarp();
       }
-      if (lane == 0) {
-        a.row_loss[row] = loss;
-        a.stats[row] = RowStats{h.m, h.s, t.tm, t.ts};
-      }
-      __syncwarp();
+      if (row >= a.rows) break;
+      before = row;
     }
   } else {
     const int tid = threadIdx.x;
-    Consumers team(sm.red);
+    Consumers<CW> team(sm.red);
     int st = 0, slot = 0;
     uint32_t phase = 0, told = 0, joins = 0;
     for (long long row = row0; row < a.rows; row += grid) {
@@ -830,10 +885,12 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
             const uint4* buf = reinterpret_cast<const uint4*>(ring + (size_t)st * CHUNK);
             const int n = o.vecs - i * (CHUNK / 16);
             uint4 u[PER];
+            if (n >= CHUNK / 16) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              const int v = tid + j * CTHREADS;
-              u[j] = v < n ? buf[v] : E::none();
+              for (int j = 0; j < PER; ++j) u[j] = buf[tid + j * CTHREADS];
+            } else {
+#pragma unroll
+              for (int j = 0; j < PER; ++j) u[j] = tid + j * CTHREADS < n ? buf[tid + j * CTHREADS] : E::none();
             }
             if (MODE == DISTILL_LOSS || !a.resident) {
               __syncwarp();
@@ -852,7 +909,7 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
             if (tid < parts) send_async(&sm.part[set][part], make_float2(r.m, r.s), &sm.joined[set], tid);
             mbar_wait_cluster(&sm.joined[set], joins >> 1 & 1, &sm.failed);
             ++joins;
-            r = Consumers::join_of(sm.part[set][lane % parts], parts, a.c);
+            r = Consumers<CW>::join_of(sm.part[set][lane % parts], parts, a.c);
           }
           m = r.m, s = r.s;
           if (far_off(m, a.c)) {  // every part over the whole row: rare, and needs no exchange
@@ -866,7 +923,7 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
         }
         if (MODE != DISTILL_LOSS) {
           const Expo ex(m, a.c);
-          const float G = h.G, gs = G / s;
+          const float G = h.G, gs = G * rcp_nr(s);
           int s2 = MODE == DISTILL_BOTH && a.resident ? st0 : st;
           for (int i = 0; i < chunks; ++i) {
             if (MODE == DISTILL_GRAD || !a.resident) mbar_wait(&sm.full[s2], phase, &sm.failed);
@@ -874,16 +931,17 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
             const int first = i * (CHUNK / 16), n = o.vecs - first;
             uint4 u[PER];
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              const int v = tid + j * CTHREADS;
-              if (v < n) u[j] = buf[v];
-            }
+            for (int j = 0; j < PER; ++j) u[j] = buf[tid + j * CTHREADS];  // behind the row's end: not used
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.empty[s2]);
+            uint4* to = gv + first + tid;
+            if (n >= CHUNK / 16) {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              const int v = tid + j * CTHREADS;
-              if (v < n) gv[first + v] = ex.scaled<T>(u[j], gs);
+              for (int j = 0; j < PER; ++j) to[j * CTHREADS] = ex.scaled<T>(u[j], gs);
+            } else {
+#pragma unroll
+              for (int j = 0; j < PER; ++j)
+                if (tid + j * CTHREADS < n) to[j * CTHREADS] = ex.scaled<T>(u[j], gs);
             }
             if (++s2 == a.stages) {
               s2 = 0;
@@ -898,7 +956,7 @@ __global__ void __launch_bounds__(CTHREADS + 32 + 32 * MAX_TELLERS, 2) distill_s
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&sm.freed[slot]);
-      if (++slot == a.tellers) slot = 0, told ^= 1;
+      if (++slot == 2 * a.tellers) slot = 0, told ^= 1;
     }
   }
   if (parts > 1)
@@ -991,7 +1049,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
   }
   if (MODE == DISTILL_LOSS) return;
   const float G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);  // NaN for a row with invalid entries
-  const float gs = G / st.s;
+  const float gs = G * rcp_nr(st.s);
   {
     const Span o = span_of(g, lo, hi);
     const int at = edge_of<T>(o, tid);
@@ -1040,7 +1098,8 @@ static int distill_check(const lpmm_b200_distill* d, int mode) {
   if (d->index_bits != 32 && d->index_bits != 64) return LPMM_B200_ERR_BAD_KIND;
   if (d->reduction < 0 || d->reduction > 2) return LPMM_B200_ERR_BAD_KIND;
   if (!(d->temperature >= LPMM_B200_DISTILL_MIN_T && d->temperature <= LPMM_B200_DISTILL_MAX_T)) return LPMM_B200_ERR_BAD_SIZE;
-  if (d->k > MAX_K || d->vocab > (1 << 30) || d->rows >= (1ll << 28)) return LPMM_B200_ERR_TOO_LARGE;
+  if (d->k > MAX_K || d->vocab > (1 << 30) || d->rows >= (1ll << 28) ||
+      d->inner >= (1ll << 28)) return LPMM_B200_ERR_TOO_LARGE;
   if (d->rows && (!d->logits || !d->teacher || !d->index || !d->work)) return LPMM_B200_ERR_NULL_POINTER;
   if (d->rows && mode != DISTILL_LOSS && !d->grad) return LPMM_B200_ERR_NULL_POINTER;
   if (mode != DISTILL_GRAD && !d->loss && (d->rows || d->reduction != LPMM_B200_REDUCE_NONE)) return LPMM_B200_ERR_NULL_POINTER;
@@ -1084,17 +1143,18 @@ static cudaError_t launch(K kernel, const DistillArgs& a, long long grid, int th
 }
 
 // how many clusters of `parts` CTAs the GPU holds at a time (asked once per kernel, size and device)
-template <typename T, int MODE>
+template <typename T, int MODE, int CW>
 static int most_clusters(int parts, int threads, size_t smem) {
-  const auto kernel = distill_stream_kernel<T, MODE>;
+  const auto kernel = distill_stream_kernel<T, MODE, CW>;
   static std::atomic<int> known[64][4][MAX_TELLERS + 1];  // 0: not asked yet
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  std::atomic<int>& n = known[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3][(threads - CTHREADS - 32) / 32];
+  std::atomic<int>& n = known[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3][threads / 32 - CW - 1];
   if (n.load() == 0) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(2 * num_sms() / parts * parts), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem;
+    cfg.gridDim = dim3(Shape<MODE, CW>::CTAS * num_sms() / parts * parts), cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = parts, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
@@ -1106,6 +1166,31 @@ static int most_clusters(int parts, int threads, size_t smem) {
   return n.load();
 }
 
+template <typename T, int MODE, int CW>
+static cudaError_t stream_launch(DistillArgs& a, long long row_bytes, bool after, cudaStream_t stream) {
+  using S = Shape<MODE, CW>;
+  const size_t fixed = (sizeof(StreamSmem) + 15) / 16 * 16, told = entry_bytes(2 * a.k_pad, a.hash_size);
+  a.tellers = S::TELLERS;
+  while (a.tellers > 1 && a.tellers * told > S::ROOM / 6) --a.tellers;
+  a.stages = (int)((S::ROOM - fixed - a.tellers * told) / S::CHUNK);
+  if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
+  // With both passes in one call a row stays in the ring where it fits.  Up to 128 KB it is else copied a second time: the
+  // rows under way are then less than 38 MB and still in L2 (bf16, 65536 columns: 214 us, and 235 shared by a cluster).
+  // Larger rows would come from memory again; clusters of CTAs share their columns (131072: 246, and 268 copied twice).
+  const long long room = (long long)(a.stages - 1) * S::CHUNK;
+  int parts = 1;
+  if (MODE == DISTILL_BOTH && row_bytes > 128 * 1024)
+    while (parts < MAX_PARTS && row_bytes > parts * room) parts *= 2;
+  const size_t smem = a.stages * S::CHUNK + fixed + a.tellers * told;
+  const int threads = S::THREADS + 32 + 32 * a.tellers;
+  const int clusters = parts > 1 ? most_clusters<T, MODE, CW>(parts, threads, smem) : S::CTAS * num_sms();
+  if (clusters <= 0) return cudaErrorInvalidConfiguration;
+  a.slice = ((a.vocab + parts - 1) / parts + 63) / 64 * 64;
+  a.resident = MODE == DISTILL_BOTH && row_bytes <= parts * room;
+  return launch(distill_stream_kernel<T, MODE, CW>, a, (a.rows < clusters ? a.rows : clusters) * parts, threads, smem, parts,
+                after, stream);
+}
+
 // `after`: the kernel before it in the stream is this call's sum of the weights
 template <typename T, int MODE>
 static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t stream) {
@@ -1113,40 +1198,31 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   const long long row_bytes = (long long)a.vocab * sizeof(T);
   const size_t entries = entry_bytes(a.k_pad, a.hash_size);
   const int sms = num_sms();
-  constexpr size_t LIMIT = 113 * 1024;  // two CTAs per SM
-  if (row_bytes <= ROWS_MAX_BYTES && a.k <= 256) {
-    a.slot = (int)(row_bytes / 16 * 16);
-    int warps = ROWS_MAX_WARPS;
+  // A warp per row up to 16 KB for the loss (bf16, 8192 columns: 171 us against 179 of the streaming kernel; fp32, 4096: 128
+  // against 165), up to 8 KB with the gradient (4096 columns: 309 against 375; 8192: 420 against 309).
+  if (row_bytes <= (MODE == DISTILL_LOSS ? ROWS_MAX_BYTES : ROWS_MAX_BYTES / 2) && a.k <= 256) {
+    a.slot = (int)((row_bytes + 15) / 16 * 16);
+    int warps = ROWS_MAX_WARPS, ctas = a.k <= 64 ? 3 : 2;
     a.stages = ROWS_MAX_STAGES;
-    const auto bytes = [&] { return (size_t)warps * (a.stages * (size_t)a.slot + 4 * (size_t)a.hash_size); };
-    while (a.stages > 2 && bytes() > LIMIT) --a.stages;
-    while (bytes() > LIMIT) --warps;
+    const auto bytes = [&] { return (size_t)warps * a.stages * a.slot; };
+    const auto room = [&] { return (size_t)(227 * 1024 / ctas - 2048); };
+    while (a.stages > 2 && bytes() > room()) --a.stages;
+    if (bytes() > room()) ctas = 2;
+    while (bytes() > room()) --warps;
     long long grid = (a.rows + warps - 1) / warps;
-    if (grid > 2 * sms) grid = 2 * sms;
+    if (grid > ctas * sms) grid = ctas * sms;
     if (a.k <= 64) return launch(distill_rows_kernel<T, MODE, 2>, a, grid, warps * 32, bytes(), 1, after, stream);
     return launch(distill_rows_kernel<T, MODE, 8>, a, grid, warps * 32, bytes(), 1, after, stream);
   }
-  if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES) {
-    const size_t fixed = (sizeof(StreamSmem) + 15) / 16 * 16;
-    a.tellers = MAX_TELLERS;
-    while (a.tellers > 1 && a.tellers * entries > 24 * 1024) --a.tellers;
-    a.stages = (int)((LIMIT - fixed - a.tellers * entries) / CHUNK);
-    if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
-    // with both passes in one call a row is to stay in the ring: large rows are shared by the CTAs of a cluster
-    const long long room = (long long)(a.stages * 3 / 4) * CHUNK;
-    int parts = 1;
-    if (MODE == DISTILL_BOTH)
-      while (parts < MAX_PARTS && row_bytes > parts * room) parts *= 2;
-    const size_t smem = a.stages * CHUNK + fixed + a.tellers * entries;
-    const int threads = CTHREADS + 32 + 32 * a.tellers;
-    const auto kernel = distill_stream_kernel<T, MODE>;
-    const int clusters = parts > 1 ? most_clusters<T, MODE>(parts, threads, smem) : 2 * sms;
-    if (clusters > 0) {
-      a.slice = ((a.vocab + parts - 1) / parts + 63) / 64 * 64;
-      a.resident = MODE == DISTILL_BOTH && row_bytes <= parts * room;
-      const long long grid = a.rows < clusters ? a.rows : clusters;
-      return launch(kernel, a, grid * parts, threads, smem, parts, after, stream);
-    }
+  if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES / 2) {
+    // Four consuming warps per CTA or eight, measured with 64 entries and 512 MB of logits (us, four / eight): the loss of
+    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; gradient 12000 194 / 200,
+    // 131072 196 / 190; both 8192 309 / -, 12000 296 / 355, 20000 270 / 292, 32000 236 / 237, 50257 255 / 233, fp32 12000
+    // 221 / 204.  Many entries take the room of the smaller ring.
+    const bool few = a.k <= 256 && row_bytes <= (MODE == DISTILL_BOTH ? 40 * 1024 : 128 * 1024);
+    const cudaError_t e = few ? stream_launch<T, MODE, 4>(a, row_bytes, after, stream)
+                              : stream_launch<T, MODE, 8>(a, row_bytes, after, stream);
+    if (e != cudaErrorInvalidConfiguration) return e;
   }
   // few rows: their columns are shared by clusters of up to 8 CTAs, so that all SMs have work
   int parts = 1;

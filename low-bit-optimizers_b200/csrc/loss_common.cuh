@@ -107,6 +107,13 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// log2 by the hardware instruction (absolute error 2^-22 near 1, relative elsewhere)
+__device__ __forceinline__ float lg2(float x) {
+  float r;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 __device__ __forceinline__ float load_any(const void* p, long long i, int dtype) {
   if (dtype == LPMM_B200_DTYPE_FP32) return reinterpret_cast<const float*>(p)[i];
   if (dtype == LPMM_B200_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
@@ -131,25 +138,27 @@ __device__ __forceinline__ void mbar_arrive(unsigned long long* b) {
 __device__ __forceinline__ void mbar_expect(unsigned long long* b, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_at(b)), "r"(bytes) : "memory");
 }
+// A wait is a matter of microseconds.  One try sleeps for up to WAIT_NS, the limit is some seconds of tries.
+constexpr uint32_t WAIT_NS = 20000;
+constexpr int WAIT_LIMIT = 1 << 18;
 __device__ __forceinline__ bool mbar_test(unsigned long long* b, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
-      : "r"(smem_at(b)), "r"(parity)
+      : "r"(smem_at(b)), "r"(parity), "r"(WAIT_NS)
       : "memory");
   return done;
 }
 __device__ __forceinline__ bool mbar_test_cluster(unsigned long long* b, uint32_t parity) {
   uint32_t done;
   asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
       : "=r"(done)
-      : "r"(smem_at(b)), "r"(parity)
+      : "r"(smem_at(b)), "r"(parity), "r"(WAIT_NS)
       : "memory");
   return done;
 }
-constexpr int WAIT_LIMIT = 1 << 22;  // tries, each of which may sleep for a while: seconds, where a wait is microseconds
 // Waits for the phase; gives up when the limit is reached or another thread of the CTA has given up (*failed).  The
 // caller goes on in either case (its data are then worthless, its accesses in range) and the kernel ends as it should.
 __device__ __forceinline__ void mbar_wait(unsigned long long* b, uint32_t parity, int* failed) {
@@ -178,6 +187,9 @@ __device__ __forceinline__ void mbar_wait_landed(unsigned long long* b, uint32_t
   for (int i = 0; i < WAIT_LIMIT; ++i)
     if (mbar_test(b, parity)) return;
 }
+// between a thread's own accesses to shared memory and a bulk copy over it that follows a barrier
+__device__ __forceinline__ void bulk_load_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 // both addresses and the size are multiples of 16 bytes
 __device__ __forceinline__ void bulk_load(void* to, const void* from, uint32_t bytes, unsigned long long* b) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_at(to)),
