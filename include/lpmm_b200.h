@@ -511,6 +511,7 @@ int lpmm_b200_distill_backward(const lpmm_b200_distill* d, void* stream);
 int lpmm_b200_distill_forward_backward(const lpmm_b200_distill* d, void* stream);
 
 #define LPMM_B200_BALANCE_MAX_EXPERTS 1024
+#define LPMM_B200_BALANCE_MAX_TOKENS (1 << 30)
 #define LPMM_B200_SCORE_SOFTMAX 0
 #define LPMM_B200_SCORE_SIGMOID 1
 
@@ -523,7 +524,8 @@ int lpmm_b200_distill_forward_backward(const lpmm_b200_distill* d, void* stream)
  * offsets[s+1]); tokens of no sequence and tokens that are not valid are not looked at and have gradient 0; a sequence
  * without valid tokens has loss 0.  A negative expert index is a dropped assignment: not counted.  An index >=
  * experts makes its sequence's loss and gradient NaN, offsets that descend or leave the range make every loss NaN;
- * nothing out of range is accessed.  Counts are whole-number atomics, sums of scores are fp32 in a fixed order. */
+ * nothing out of range is accessed.  Counts are whole-number atomics; sums of scores are fp32 within a run of tokens of
+ * one warp and 64-bit whole numbers beyond: results do not depend on how the work is scheduled. */
 typedef struct lpmm_b200_balance {
   const void* logits;      /* row r begins at element (r / inner) * outer_stride + (r % inner) * inner_stride           */
   void* grad;              /* [tokens, experts] contiguous, type of the logits (not for forward)                        */
@@ -534,7 +536,8 @@ typedef struct lpmm_b200_balance {
   float* loss;             /* [sequences] (not for backward)                                                            */
   int64_t* counts;         /* [sequences, experts]: written by forward, read by backward                                */
   float* factor;           /* [sequences]: experts / (k n^2), written by forward, read by backward                      */
-  void* work;              /* lpmm_b200_balance_work_bytes, 16-byte aligned (not for backward)                          */
+  void* work;              /* lpmm_b200_balance_work_bytes, 8-byte aligned (not for backward); directly behind counts   */
+                           /* saves a clearing operation                                                                */
   int64_t tokens, inner, outer_stride, inner_stride;
   int64_t experts, k, sequences;
   int32_t dtype, index_bits, offset_bits, score;
@@ -542,7 +545,7 @@ typedef struct lpmm_b200_balance {
   int32_t reserved;
 } lpmm_b200_balance;
 
-int64_t lpmm_b200_balance_work_bytes(int64_t tokens, int64_t experts, int64_t sequences);
+int64_t lpmm_b200_balance_work_bytes(int64_t experts, int64_t sequences);
 int lpmm_b200_balance_forward(const lpmm_b200_balance* b, void* stream);
 /* grad_scale * sum over sequences of upstream[s] * gradient of loss[s]. */
 int lpmm_b200_balance_backward(const lpmm_b200_balance* b, void* stream);

@@ -5,15 +5,21 @@
 //   F = experts / (k n^2), n = valid tokens of the sequence
 //
 // The gradient needs the counts, not the summed scores, so loss and gradient share one pass over the logits once the
-// indices are counted.  A token's logits lie in the registers of 2 ... 32 lanes; a warp walks a contiguous run of
-// tokens and sums the scores of its columns in registers.  Sums meet in a fixed order: groups of a warp by shuffles,
-// warps of a CTA in shared memory, CTAs in the last kernel; a sequence that ends inside a run is written out there.
-// Bound by memory for large batches (a logit is read once, a gradient written once), by launches for small ones.
+// indices are counted.  A token's logits lie in the registers of up to 32 lanes, some tokens per warp at a time; a warp
+// walks a contiguous run of tokens and sums the scores of its columns in registers, in fp32.  Those sums (a run has at
+// most some hundred tokens) meet as 64-bit whole numbers, in units of 2^-shift with tokens * 2^shift < 2^62: atomics on
+// them give the same result in any order, and what is rounded off is far below fp32 of the sum.
+// Bound by memory for large batches (a logit is read once, a gradient written once), by launches for small ones: these
+// are done in one launch of a CTA or a cluster, larger ones in three (clear, count, scores; the last CTA adds up).
+#include <cooperative_groups.h>
+
 #include "loss_common.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace lpmm_b200 {
 
-constexpr int WARPS = 8;
+constexpr int MAX_WARPS = 16;
 
 struct BalanceArgs {
   const void* logits;
@@ -23,208 +29,265 @@ struct BalanceArgs {
   const void* offsets;
   const float* upstream;
   float* loss;
-  unsigned long long* counts;
+  unsigned long long* counts;  // [sequences, experts]
   float* factor;
-  unsigned long long* sizes;  // valid tokens per sequence
-  int* bad;                   // per sequence: an index out of range; [sequences]: the offsets are not in order
-  float* psum;                // [sequences, experts]: sequences that lie within one CTA's tokens
-  float* partial;             // [CTAs, 2, experts]: the sequence that a CTA's first / last tokens share with others
-  long long tokens, inner, outer_stride, inner_stride, sequences, tile;
-  int experts, k, index_bits, offset_bits, sigmoid, group;
+  unsigned long long* psum;    // [sequences, experts] summed scores in units of 2^-shift
+  unsigned long long* sizes;   // valid tokens per sequence
+  int* bad;                    // per sequence: 1 an index out of range, 2 a score that is NaN; [sequences]: offsets not in order
+  unsigned* ticket;            // CTAs that are done
+  long long inner, outer_stride, inner_stride;
+  int tokens, sequences, tile, experts, k, index_bits, offset_bits, sigmoid, group, shift;
+  int finish;                  // the last CTA of the scores adds up
   float scale;
 };
 
-__device__ __forceinline__ long long raw_offset(const BalanceArgs& a, long long i) {
+__device__ __forceinline__ long long raw_offset(const BalanceArgs& a, int i) {
   if (!a.offsets) return i == 0 ? 0 : a.tokens;
   return load_index(a.offsets, i, a.offset_bits);
 }
-__device__ __forceinline__ long long offset_at(const BalanceArgs& a, long long i) {
-  return min(max(raw_offset(a, i), 0ll), a.tokens);
+__device__ __forceinline__ int offset_at(const BalanceArgs& a, int i) {
+  return (int)min(max(raw_offset(a, i), 0ll), (long long)a.tokens);
 }
 
 // The stretch of tokens from r on that belongs to one sequence: s in [0, sequences), or s < 0 for tokens of none.
 // Whatever the offsets hold, r < end <= hi and s is in range.
 struct Stretch {
-  long long s, end;
+  int s, end;
 };
-__device__ __forceinline__ Stretch stretch_at(const BalanceArgs& a, long long r, long long hi) {
+__device__ __forceinline__ Stretch stretch_at(const BalanceArgs& a, int r, int hi) {
   if (!a.offsets) return Stretch{0, hi};
-  long long lo = -1, up = a.sequences + 1;  // offset(lo) <= r < offset(up)
+  int lo = -1, up = a.sequences + 1;  // offset(lo) <= r < offset(up)
   while (up - lo > 1) {
-    const long long mid = (lo + up) >> 1;
+    const int mid = (lo + up) >> 1;
     if (offset_at(a, mid) <= r)
       lo = mid;
     else
       up = mid;
   }
-  Stretch t;
-  t.s = lo == a.sequences ? -1 : lo;
-  t.end = lo == a.sequences ? hi : max(min(offset_at(a, lo + 1), hi), r + 1);
-  return t;
+  if (lo == a.sequences) return Stretch{-1, hi};
+  return Stretch{lo, max(min(offset_at(a, lo + 1), hi), r + 1)};
 }
 
-__device__ __forceinline__ double factor_of(const BalanceArgs& a, long long s) {
-  if (a.bad[s] || a.bad[a.sequences]) return (double)nan_f();
-  const double n = (double)a.sizes[s];
+__device__ __forceinline__ long long cell(const BalanceArgs& a, int s, int e) { return (long long)s * a.experts + e; }
+
+// (what earlier phases of the same launch have written is read past L1)
+__device__ __forceinline__ double factor_of(const BalanceArgs& a, int s) {
+  if ((__ldcg(&a.bad[s]) & 1) || __ldcg(&a.bad[a.sequences])) return (double)nan_f();
+  const double n = (double)__ldcg(&a.sizes[s]);
   return n == 0.0 ? 0.0 : (double)a.experts / ((double)a.k * n * n);
 }
 
-// Assignments per expert and valid tokens per sequence.  One sequence: a histogram per CTA in shared memory; several:
-// a warp counts its run of tokens straight into the sequence's row.
-__global__ void __launch_bounds__(WARPS * 32) balance_count_kernel(const BalanceArgs a) {
-  extern __shared__ int hist[];
-  const bool one = a.sequences == 1;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (blockIdx.x == 0 && a.offsets) {
+// A CTA's part of the tokens.  What its first and its last sequence gather is put together in shared memory (they may
+// have many tokens here); sequences between them lie within the CTA and go straight to memory.
+struct Tile {
+  int lo, hi, first, last;
+  __device__ __forceinline__ Tile(const BalanceArgs& a, int cta) {
+    lo = (int)min((long long)cta * a.tile, (long long)a.tokens);
+    hi = min(lo + a.tile, a.tokens);
+    first = last = -1;
+    if (lo < hi) {
+      first = stretch_at(a, lo, hi).s;
+      last = stretch_at(a, hi - 1, hi).s;
+    }
+  }
+  // this warp's run
+  __device__ __forceinline__ void run(int& from, int& to) const {
+    const int warps = blockDim.x >> 5, n = (hi - lo + warps - 1) / warps;
+    from = min(lo + (int)(threadIdx.x >> 5) * n, hi);
+    to = min(from + n, hi);
+  }
+  __device__ __forceinline__ int set(int s) const { return s == first ? 0 : s == last ? 1 : -1; }
+};
+
+// Assignments per expert and valid tokens per sequence.  hist: int[2, experts] in shared memory
+__device__ __forceinline__ void count_phase(const BalanceArgs& a, int cta, int* hist) {
+  const int lane = threadIdx.x & 31;
+  if (cta == 0 && a.offsets) {
     bool off = false;
-    for (long long i = threadIdx.x; i <= a.sequences; i += blockDim.x) {
+    for (int i = threadIdx.x; i <= a.sequences; i += blockDim.x) {
       const long long o = raw_offset(a, i);
       off |= o < 0 || o > a.tokens || (i && raw_offset(a, i - 1) > o);
     }
     if (off) a.bad[a.sequences] = 1;
   }
-  if (one) {
-    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) hist[e] = 0;
-    __syncthreads();
-  }
-  const long long tile_lo = blockIdx.x * a.tile, tile_hi = min(tile_lo + a.tile, a.tokens);
-  const long long run = (a.tile + WARPS - 1) / WARPS;
-  const long long lo = tile_lo + warp * run, hi = min(lo + run, tile_hi);
-  for (long long r = lo; r < hi;) {
+  for (int e = threadIdx.x; e < 2 * a.experts; e += blockDim.x) hist[e] = 0;
+  const Tile tile(a, cta);
+  __syncthreads();
+  int lo, hi;
+  tile.run(lo, hi);
+  for (int r = lo; r < hi;) {
     const Stretch t = stretch_at(a, r, hi);
     if (t.s >= 0) {
+      const int set = tile.set(t.s);
       int size = 0;
-      for (long long q = r + lane; q < t.end; q += 32) size += !a.valid || a.valid[q];
-      size = __reduce_add_sync(~0u, size);
-      if (lane == 0 && size) atomicAdd(&a.sizes[t.s], (unsigned long long)size);
-      for (long long q = r * a.k + lane; q < t.end * a.k; q += 32) {
-        if (a.valid && !a.valid[q / a.k]) continue;
-        const long long e = load_index(a.index, q, a.index_bits);
-        if (e < 0) continue;
-        if (e >= a.experts)
-          a.bad[t.s] = 1;
-        else if (one)
-          atomicAdd(&hist[e], 1);
-        else
-          atomicAdd(&a.counts[t.s * a.experts + e], 1ull);
+      for (int q = r; q < t.end; q += 32) {  // 32 tokens at a time
+        const int n = min(32, t.end - q);
+        const unsigned ok = __ballot_sync(~0u, lane < n && (!a.valid || a.valid[q + lane]));
+        size += __popc(ok);
+        const long long first = (long long)q * a.k;
+        const int entries = n * a.k;
+        for (int i = lane; i < entries; i += 32 * 4) {
+          long long e[4];
+#pragma unroll
+          for (int u = 0; u < 4; ++u) e[u] = i + 32 * u < entries ? load_index(a.index, first + i + 32 * u, a.index_bits) : -1;
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            if (e[u] < 0 || (a.valid && !(ok >> ((unsigned)(i + 32 * u) / (unsigned)a.k) & 1))) continue;
+            if (e[u] >= a.experts)
+              atomicOr(&a.bad[t.s], 1);
+            else if (set >= 0)
+              atomicAdd(&hist[set * a.experts + (int)e[u]], 1);
+            else
+              atomicAdd(&a.counts[cell(a, t.s, (int)e[u])], 1ull);
+          }
+        }
       }
+      if (lane == 0 && size) atomicAdd(&a.sizes[t.s], (unsigned long long)size);
     }
     r = t.end;
   }
-  if (one) {
-    __syncthreads();
-    for (int e = threadIdx.x; e < a.experts; e += blockDim.x)
-      if (hist[e]) atomicAdd(&a.counts[e], (unsigned long long)hist[e]);
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+    if (tile.first >= 0 && hist[e]) atomicAdd(&a.counts[cell(a, tile.first, e)], (unsigned long long)hist[e]);
+    if (tile.last >= 0 && hist[a.experts + e])
+      atomicAdd(&a.counts[cell(a, tile.last, e)], (unsigned long long)hist[a.experts + e]);
   }
 }
 
 // Scores of all tokens: their sums (SUM), the gradient (GRAD).  V: elements per load (16 bytes, or 1 where rows are
-// not 16-byte aligned), J: loads per lane; a.group lanes (a power of two) hold a token's logits.
-template <typename T, int V, int J, bool SUM, bool GRAD>
-__global__ void __launch_bounds__(WARPS * 32) balance_kernel(const BalanceArgs a) {
+// not 16-byte aligned), J: loads per lane; a.group lanes (a power of two) hold a token's logits, U tokens each are under
+// way at a time.  sums: unsigned long long[2, experts] in shared memory
+template <typename T, int V, int J, bool SIG, bool SUM, bool GRAD>
+__device__ __forceinline__ void score_phase(const BalanceArgs& a, int cta, unsigned long long* sums) {
   using E = Elem<T>;
-  extern __shared__ float slots[];  // [WARPS, 2, experts]
-  __shared__ long long owner[WARPS][2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  constexpr int U = J * V <= 8 ? (SIG ? 2 : 4) : J * V <= 16 && !SIG ? 2 : 1;
+  const int lane = threadIdx.x & 31;
   const int G = a.group, per = 32 / G, gl = lane & (G - 1), gi = lane / G;
-  const long long tile_lo = blockIdx.x * a.tile, tile_hi = min(tile_lo + a.tile, a.tokens);
-  const long long run = (a.tile + WARPS - 1) / WARPS;
-  const long long lo = tile_lo + warp * run, hi = min(lo + run, tile_hi);
-  if (SUM && threadIdx.x < WARPS * 2) owner[threadIdx.x >> 1][threadIdx.x & 1] = -1;
+  if (SUM)
+    for (int e = threadIdx.x; e < 2 * a.experts; e += blockDim.x) sums[e] = 0;
+  const Tile tile(a, cta);
   if (SUM) __syncthreads();
+  int lo, hi;
+  tile.run(lo, hi);
   constexpr float LOG2E = 1.4426950408889634f;
-  const float minus_inf = -__int_as_float(0x7f800000);
+  const float minus_inf = -__int_as_float(0x7f800000), units = __int_as_float((a.shift + 127) << 23);
 
-  for (long long r0 = lo; r0 < hi;) {
+  for (int r0 = lo; r0 < hi;) {
     const Stretch t = stretch_at(a, r0, hi);
     float c[J * V], acc[J * V], fac = 0.0f;
-    if (GRAD) {
-      if (t.s >= 0) {
-        fac = a.scale * (SUM ? (float)factor_of(a, t.s) : a.factor[t.s] * a.upstream[t.s]);
+    if (GRAD && t.s >= 0) {
+      fac = a.scale * (SUM ? (float)factor_of(a, t.s) : a.factor[t.s] * a.upstream[t.s]);
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+      for (int j = 0; j < J; ++j)
 #pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const int col = (j * G + gl) * V + i;
-            c[j * V + i] = col < a.experts ? (float)a.counts[t.s * a.experts + col] : 0.0f;
-          }
-      }
+        for (int i = 0; i < V; ++i) {
+          const int col = (j * G + gl) * V + i;
+          c[j * V + i] = col < a.experts ? (float)__ldcg(&a.counts[cell(a, t.s, col)]) : 0.0f;
+        }
     }
 #pragma unroll
     for (int i = 0; i < J * V; ++i) acc[i] = 0.0f;
-    for (long long base = r0; base < t.end; base += per) {
-      const long long r = base + gi;
-      const bool here = r < t.end, ok = here && t.s >= 0 && (!a.valid || a.valid[r]);
-      float x[J * V];
-      const T* row = reinterpret_cast<const T*>(a.logits) + (r / a.inner) * a.outer_stride + (r % a.inner) * a.inner_stride;
-      float m = minus_inf;
+    for (int base = r0; base < t.end; base += per * U) {
+      bool here[U], ok[U];
+      float x[U][J * V], m[U], sum[U];
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        const int col = (j * G + gl) * V;
-        if (ok && col < a.experts) {
-          if (V == 1)
-            x[j] = E::widen(row[col]);
-          else
-            E::unpack(*reinterpret_cast<const uint4*>(row + col), x + j * V);
-        } else {
-#pragma unroll
-          for (int i = 0; i < V; ++i) x[j * V + i] = ok ? minus_inf : 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) m = fmaxf(m, x[j * V + i]);
-      }
-      for (int d = G >> 1; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, d));
-      // p holds the score, x (sigmoid only) 1 - sigmoid
-      float p[J * V], sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < J * V; ++i) {
-        if (a.sigmoid) {
-          // sigmoid(x) = e^min(x,0) / (1 + e^-|x|), scaled by e^-min(m,0) so that the largest one stays near 1
-          const float fall = ex2(-fabsf(x[i]) * LOG2E), d = __frcp_rn(1.0f + fall);
-          p[i] = ex2((fminf(x[i], 0.0f) - fminf(m, 0.0f)) * LOG2E) * d;
-          if (!(x[i] == x[i])) p[i] = x[i];
-          x[i] = x[i] >= 0.0f ? fall * d : d;
-        } else {
-          p[i] = ex2((x[i] - m) * LOG2E);
-        }
-        sum += p[i];
-      }
-      for (int d = G >> 1; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
-      const float inv = __frcp_rn(sum);
-      float dot = 0.0f;
-#pragma unroll
-      for (int i = 0; i < J * V; ++i) {
-        p[i] *= inv;
-        if (SUM) acc[i] += ok ? p[i] : 0.0f;
-        if (GRAD) dot = fmaf(c[i], p[i], dot);
-      }
-      if (GRAD) {
-        for (int d = G >> 1; d; d >>= 1) dot += __shfl_xor_sync(~0u, dot, d);
-        T* g = reinterpret_cast<T*>(a.grad) + r * a.experts;
+      for (int u = 0; u < U; ++u) {
+        const int r = base + u * per + gi;
+        here[u] = r < t.end;
+        ok[u] = here[u] && t.s >= 0 && (!a.valid || a.valid[r]);
+        const T* row = reinterpret_cast<const T*>(a.logits) + row_at(r, a.inner, a.outer_stride, a.inner_stride);
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           const int col = (j * G + gl) * V;
-          if (here && col < a.experts) {
+          const bool in = ok[u] && col < a.experts;
+          if constexpr (V == 1) {
+            x[u][j] = in ? E::widen(row[col]) : ok[u] ? minus_inf : 0.0f;
+          } else {
+            const uint4 w = in ? *reinterpret_cast<const uint4*>(row + col) : ok[u] ? E::none() : make_uint4(0, 0, 0, 0);
+            E::unpack(w, x[u] + j * V);
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        m[u] = x[u][0];
+#pragma unroll
+        for (int i = 1; i < J * V; ++i) m[u] = fmaxf(m[u], x[u][i]);
+      }
+      for (int d = G >> 1; d; d >>= 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(~0u, m[u], d));
+      }
+      // p: the score; x (sigmoid only): 1 - sigmoid
+      float p[U][J * V];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        sum[u] = 0.0f;
+        if constexpr (SIG) {
+          // sigmoid(x) = e^min(x,0) / (1 + e^-|x|), scaled by e^-min(m,0) so that the largest one stays near 1
+          const float top = fminf(m[u], 0.0f);
+#pragma unroll
+          for (int i = 0; i < J * V; ++i) {
+            const float v = x[u][i], fall = ex2(-fabsf(v) * LOG2E), d = rcp_nr(1.0f + fall);
+            p[u][i] = v == v ? ex2((fminf(v, 0.0f) - top) * LOG2E) * d : v;
+            x[u][i] = v >= 0.0f ? fall * d : d;
+            sum[u] += p[u][i];
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < J * V; ++i) {
+            p[u][i] = ex2((x[u][i] - m[u]) * LOG2E);
+            sum[u] += p[u][i];
+          }
+        }
+      }
+      for (int d = G >> 1; d; d >>= 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) sum[u] += __shfl_xor_sync(~0u, sum[u], d);
+      }
+      float dot[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float inv = rcp_nr(sum[u]);
+        dot[u] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < J * V; ++i) {
+          p[u][i] *= inv;
+          if (SUM) acc[i] += ok[u] ? p[u][i] : 0.0f;
+          if (GRAD) dot[u] = fmaf(c[i], p[u][i], dot[u]);
+        }
+      }
+      if (GRAD) {
+        for (int d = G >> 1; d; d >>= 1) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) dot[u] += __shfl_xor_sync(~0u, dot[u], d);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          T* g = reinterpret_cast<T*>(a.grad) + (long long)(base + u * per + gi) * a.experts;
+#pragma unroll
+          for (int j = 0; j < J; ++j) {
+            const int col = (j * G + gl) * V;
             float y[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-              float v = fac * p[j * V + i] * (c[j * V + i] - dot);
-              if (a.sigmoid) v *= x[j * V + i];
-              y[i] = ok ? v : 0.0f;
+              float v = fac * p[u][j * V + i] * (c[j * V + i] - dot[u]);
+              if (SIG) v *= x[u][j * V + i];
+              y[i] = ok[u] ? v : 0.0f;
             }
-            if (V == 1)
-              g[col] = E::narrow(y[0]);
-            else
-              *reinterpret_cast<uint4*>(g + col) = E::pack(y);
+            if (here[u] && col < a.experts) {
+              if constexpr (V == 1)
+                g[col] = E::narrow(y[0]);
+              else
+                *reinterpret_cast<uint4*>(g + col) = E::pack(y);
+            }
           }
         }
       }
     }
     if (SUM && t.s >= 0) {
-      const long long first = offset_at(a, t.s), last = offset_at(a, t.s + 1);
-      const bool whole = first >= lo && last <= hi;  // the sequence lies within this warp's run
-      const int slot = first <= lo ? 0 : 1;
-      float* to = whole ? a.psum + t.s * a.experts : slots + (warp * 2 + slot) * a.experts;
+      const int set = tile.set(t.s);
+      bool nan = false;
 #pragma unroll
       for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -232,102 +295,110 @@ __global__ void __launch_bounds__(WARPS * 32) balance_kernel(const BalanceArgs a
           float v = acc[j * V + i];
           for (int d = G; d < 32; d <<= 1) v += __shfl_xor_sync(~0u, v, d);
           const int col = (j * G + gl) * V + i;
-          if (gi == 0 && col < a.experts) to[col] = v;
+          if (gi == 0 && col < a.experts) {
+            nan |= !(v == v);
+            const unsigned long long n = (unsigned long long)__float2ll_rn(v * units);
+            if (set >= 0)
+              atomicAdd(&sums[set * a.experts + col], n);
+            else
+              atomicAdd(&a.psum[cell(a, t.s, col)], n);
+          }
         }
-      if (!whole && lane == 0) owner[warp][slot] = t.s;
+      if (nan) atomicOr(&a.bad[t.s], 2);
     }
     r0 = t.end;
   }
   if (!SUM) return;
   __syncthreads();
-  // the warps' first and last stretches, in order
   for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
-    long long s = -1;
-    float v = 0.0f;
-    for (int i = 0; i <= WARPS * 2; ++i) {
-      const long long o = i < WARPS * 2 ? owner[i >> 1][i & 1] : -1;
-      if (i < WARPS * 2 && o < 0) continue;
-      if (o != s || i == WARPS * 2) {
-        if (s >= 0) {
-          const long long first = offset_at(a, s), last = offset_at(a, s + 1);
-          if (first >= tile_lo && last <= tile_hi)
-            a.psum[s * a.experts + e] = v;
-          else
-            a.partial[((long long)blockIdx.x * 2 + (first <= tile_lo ? 0 : 1)) * a.experts + e] = v;
-        }
-        s = o;
-        v = 0.0f;
-      }
-      if (i < WARPS * 2) v += slots[i * a.experts + e];
-    }
+    if (tile.first >= 0 && sums[e]) atomicAdd(&a.psum[cell(a, tile.first, e)], sums[e]);
+    if (tile.last >= 0 && sums[a.experts + e]) atomicAdd(&a.psum[cell(a, tile.last, e)], sums[a.experts + e]);
   }
 }
 
-// One CTA per sequence: the score sums of the CTAs that shared it, the loss and the gradient's factor.
-__global__ void __launch_bounds__(256) balance_loss_kernel(const BalanceArgs a) {
-  __shared__ float part[256];
-  __shared__ double red[8];
-  const long long s = blockIdx.x;
-  const double f = factor_of(a, s);
-  const long long first = offset_at(a, s), last = offset_at(a, s + 1);
-  double sum = 0.0;
-  if (f != 0.0 && f == f) {  // uniform
-    const long long t0 = first / a.tile, t1 = (last - 1) / a.tile;
-    int cols = 32;
-    while (cols < a.experts && cols < 256) cols *= 2;
-    const int ny = 256 / cols, y = threadIdx.x / cols, cx = threadIdx.x % cols;
-    for (int e0 = 0; e0 < a.experts; e0 += cols) {
-      const int e = e0 + cx;
-      float v = 0.0f;
-      if (e < a.experts) {
-        if (t0 == t1) {
-          if (y == 0) v = a.psum[s * a.experts + e];
-        } else {
-          for (long long t = t0 + y; t <= t1; t += ny)
-            v += a.partial[(t * 2 + (first <= t * a.tile ? 0 : 1)) * a.experts + e];
-        }
-      }
-      part[threadIdx.x] = v;
-      __syncthreads();
-      if (y == 0 && e < a.experts) {
-        for (int i = 1; i < ny; ++i) v += part[i * cols + cx];
-        sum += (double)a.counts[s * a.experts + e] * (double)v;
-      }
-      __syncthreads();
-    }
-  }
+// Loss and factor of the sequences s = first, first + step, ...: one warp each.  Reads what other CTAs have written.
+__device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int step) {
+  const int lane = threadIdx.x & 31;
+  for (int s = first; s < a.sequences; s += step) {
+    double sum = 0.0;
+    for (int e = lane; e < a.experts; e += 32)
+      sum += (double)__ldcg(&a.counts[cell(a, s, e)]) * (double)__ldcg(&a.psum[cell(a, s, e)]);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = sum;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    sum = 0.0;
-    for (int i = 0; i < 8; ++i) sum += red[i];
-    a.loss[s] = (float)(sum * f);
-    a.factor[s] = (float)f;
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+    if (lane == 0) {
+      const double f = factor_of(a, s);
+      a.factor[s] = (float)f;
+      a.loss[s] = __ldcg(&a.bad[s]) & 2 ? nan_f() : (float)(sum * f * exp2(-(double)a.shift));
+    }
   }
 }
 
-// workspace: sizes, bad (cleared before each call), psum, partial; 16-byte aligned parts
+__global__ void __launch_bounds__(256) balance_count_kernel(const BalanceArgs a) {
+  extern __shared__ unsigned long long shared[];
+  pdl_start_next();
+  count_phase(a, blockIdx.x, reinterpret_cast<int*>(shared));
+}
+
+template <typename T, int V, int J, bool SIG, bool SUM, bool GRAD>
+__global__ void __launch_bounds__(256, J * V <= 8 ? 3 : 2) balance_score_kernel(const BalanceArgs a) {
+  extern __shared__ unsigned long long shared[];
+  __shared__ bool last;
+  pdl_wait();
+  score_phase<T, V, J, SIG, SUM, GRAD>(a, blockIdx.x, shared);
+  if (SUM && a.finish) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1u) == gridDim.x - 1;
+    __syncthreads();
+    if (last) {
+      __threadfence();
+      loss_phase(a, threadIdx.x >> 5, blockDim.x >> 5);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(256) balance_loss_kernel(const BalanceArgs a) {
+  loss_phase(a, (blockIdx.x * blockDim.x + threadIdx.x) >> 5, gridDim.x * (blockDim.x >> 5));
+}
+
+// Everything in one launch of one cluster (of one CTA, where that is enough).
+template <typename T, int V, int J, bool SIG, bool GRAD>
+__global__ void __launch_bounds__(MAX_WARPS * 32, 1) balance_small_kernel(const BalanceArgs a) {
+  extern __shared__ unsigned long long shared[];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  const auto all = [&] {
+    __threadfence();
+    if (ctas > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+  };
+  const long long cells = (long long)a.sequences * a.experts, id = (long long)cta * blockDim.x + threadIdx.x;
+  for (long long i = id; i < cells; i += ctas * blockDim.x) a.counts[i] = a.psum[i] = 0;
+  for (long long i = id; i <= a.sequences; i += ctas * blockDim.x) {
+    if (i < a.sequences) a.sizes[i] = 0;
+    a.bad[i] = 0;
+  }
+  all();
+  count_phase(a, cta, reinterpret_cast<int*>(shared));
+  all();
+  score_phase<T, V, J, SIG, true, GRAD>(a, cta, shared);
+  all();
+  loss_phase(a, (int)(id >> 5), ctas * (blockDim.x >> 5));
+}
+
+// workspace: psum, sizes, bad, ticket
 struct BalanceLayout {
-  int64_t ctas, tile, bad_at, psum_at, partial_at, bytes;
+  int64_t sizes_at, bad_at, ticket_at, bytes;
 };
 
-static BalanceLayout balance_layout(int64_t tokens, int64_t experts, int64_t sequences) {
+static BalanceLayout balance_layout(int64_t experts, int64_t sequences) {
   BalanceLayout l;
-  int64_t ctas = (tokens + 4 * WARPS - 1) / (4 * WARPS);
-  const int64_t most = 2 * 148;
-  if (ctas > most) ctas = most;
-  if (ctas < 1) ctas = 1;
-  l.tile = (tokens + ctas - 1) / ctas;
-  if (l.tile < 1) l.tile = 1;
-  l.ctas = (tokens + l.tile - 1) / l.tile;
-  if (l.ctas < 1) l.ctas = 1;
-  auto up = [](int64_t v) { return (v + 15) / 16 * 16; };
-  l.bad_at = up(8 * sequences);
-  l.psum_at = l.bad_at + up(4 * (sequences + 1));
-  l.partial_at = l.psum_at + up(4 * sequences * experts);
-  l.bytes = l.partial_at + 4 * l.ctas * 2 * experts;
+  l.sizes_at = 8 * sequences * experts;
+  l.bad_at = l.sizes_at + 8 * sequences;
+  l.ticket_at = l.bad_at + 4 * (sequences + 1);
+  l.bytes = (l.ticket_at + 4 + 15) / 16 * 16;
   return l;
 }
 
@@ -339,48 +410,83 @@ static int balance_check(const lpmm_b200_balance* b, bool sum, bool grad) {
   if (b->score != LPMM_B200_SCORE_SOFTMAX && b->score != LPMM_B200_SCORE_SIGMOID) return LPMM_B200_ERR_BAD_KIND;
   if (b->offsets ? b->offset_bits != 32 && b->offset_bits != 64 : b->sequences != 1) return LPMM_B200_ERR_BAD_KIND;
   if (b->experts > LPMM_B200_BALANCE_MAX_EXPERTS || b->k > LPMM_B200_BALANCE_MAX_EXPERTS ||
-      b->tokens > (1ll << 40) || b->sequences >= (1ll << 31) - 1)
+      b->tokens > LPMM_B200_BALANCE_MAX_TOKENS || b->inner > (1ll << 30) || b->sequences > (1 << 24))
     return LPMM_B200_ERR_TOO_LARGE;
   if (!b->counts || !b->factor) return LPMM_B200_ERR_NULL_POINTER;
   if (b->tokens && (!b->logits || (sum && !b->index) || (grad && !b->grad))) return LPMM_B200_ERR_NULL_POINTER;
   if (sum && (!b->loss || !b->work)) return LPMM_B200_ERR_NULL_POINTER;
   if (!sum && !b->upstream) return LPMM_B200_ERR_NULL_POINTER;
-  if (sum && ((uintptr_t)b->work & 15)) return LPMM_B200_ERR_BAD_SIZE;
+  if (sum && ((uintptr_t)b->work & 7)) return LPMM_B200_ERR_BAD_SIZE;
   return LPMM_B200_OK;
 }
 
-template <typename T, int V, int J, bool SUM, bool GRAD>
-static cudaError_t balance_launch(const BalanceArgs& a, int64_t ctas, cudaStream_t stream) {
-  const size_t smem = SUM ? sizeof(float) * WARPS * 2 * a.experts : 0;
-  if (smem > 40 * 1024) {
-    cudaError_t e = cudaFuncSetAttribute(balance_kernel<T, V, J, SUM, GRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)smem);
-    if (e != cudaSuccess) return e;
+template <typename K>
+static cudaError_t balance_launch(K kernel, const BalanceArgs& a, int ctas, int threads, size_t smem, int cluster, bool after,
+                                  cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas), cfg.blockDim = dim3(threads), cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
+  if (cluster > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = cluster;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
   }
-  balance_kernel<T, V, J, SUM, GRAD><<<(unsigned)ctas, WARPS * 32, smem, stream>>>(a);
-  return cudaGetLastError();
+  if (after) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs].val.programmaticStreamSerializationAllowed = 1;
+    ++cfg.numAttrs;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, a);
+}
+
+constexpr int SMALL_CLUSTER = 8;
+constexpr int64_t SMALL_WORK = 32768;  // logits per CTA up to which one launch is quicker than three
+
+// ctas < 0: everything in one launch of a cluster of -ctas
+template <typename T, int V, int J, bool SUM, bool GRAD>
+static cudaError_t balance_scores(const BalanceArgs& a, int ctas, cudaStream_t stream) {
+  const size_t smem = SUM ? 16 * (size_t)a.experts : 0;
+  if constexpr (SUM && J * V <= 8) {
+    if (ctas < 0)
+      return a.sigmoid
+                 ? balance_launch(balance_small_kernel<T, V, J, true, GRAD>, a, -ctas, MAX_WARPS * 32, smem, -ctas, false, stream)
+                 : balance_launch(balance_small_kernel<T, V, J, false, GRAD>, a, -ctas, MAX_WARPS * 32, smem, -ctas, false, stream);
+  }
+  return a.sigmoid ? balance_launch(balance_score_kernel<T, V, J, true, SUM, GRAD>, a, ctas, 256, smem, 1, SUM, stream)
+                   : balance_launch(balance_score_kernel<T, V, J, false, SUM, GRAD>, a, ctas, 256, smem, 1, SUM, stream);
+}
+
+// 16-byte loads where every row (and row of the gradient) begins on a 16-byte boundary
+static bool balance_wide(const lpmm_b200_balance* b, bool grad) {
+  const int64_t ve = b->dtype == LPMM_B200_DTYPE_FP32 ? 4 : 8;
+  return b->experts % ve == 0 && ((uintptr_t)b->logits & 15) == 0 && (!grad || ((uintptr_t)b->grad & 15) == 0) &&
+         b->outer_stride % ve == 0 && b->inner_stride % ve == 0;
+}
+// values per lane
+static int balance_per_lane(const lpmm_b200_balance* b, bool wide) {
+  const int ve = !wide ? 1 : b->dtype == LPMM_B200_DTYPE_FP32 ? 4 : 8;
+  return (int)((b->experts + 32 * ve - 1) / (32 * ve)) * ve;
 }
 
 template <typename T, bool SUM, bool GRAD>
-static cudaError_t balance_shape(BalanceArgs& a, int64_t ctas, cudaStream_t stream) {
+static cudaError_t balance_shape(BalanceArgs& a, bool wide, int ctas, cudaStream_t stream) {
   constexpr int VE = Elem<T>::VE;
-  // 16-byte loads where every row (and row of the gradient) begins on a 16-byte boundary
-  const bool wide = a.experts % VE == 0 && ((uintptr_t)a.logits & 15) == 0 && (!GRAD || ((uintptr_t)a.grad & 15) == 0) &&
-                    a.outer_stride % VE == 0 && a.inner_stride % VE == 0;
   const int loads = wide ? a.experts / VE : a.experts;
   a.group = 1;
   while (a.group < loads && a.group < 32) a.group *= 2;
   const int j = (loads + 31) / 32;
   if (wide) {
-    if (j <= 1) return balance_launch<T, VE, 1, SUM, GRAD>(a, ctas, stream);
-    if (j <= 2) return balance_launch<T, VE, 2, SUM, GRAD>(a, ctas, stream);
-    if (j <= 4) return balance_launch<T, VE, 4, SUM, GRAD>(a, ctas, stream);
-    return balance_launch<T, VE, 8, SUM, GRAD>(a, ctas, stream);
+    if (j <= 1) return balance_scores<T, VE, 1, SUM, GRAD>(a, ctas, stream);
+    if (j <= 2) return balance_scores<T, VE, 2, SUM, GRAD>(a, ctas, stream);
+    if (j <= 4) return balance_scores<T, VE, 4, SUM, GRAD>(a, ctas, stream);
+    if constexpr (VE == 4) return balance_scores<T, VE, 8, SUM, GRAD>(a, ctas, stream);
   }
-  if (j <= 1) return balance_launch<T, 1, 1, SUM, GRAD>(a, ctas, stream);
-  if (j <= 4) return balance_launch<T, 1, 4, SUM, GRAD>(a, ctas, stream);
-  if (j <= 16) return balance_launch<T, 1, 16, SUM, GRAD>(a, ctas, stream);
-  return balance_launch<T, 1, 32, SUM, GRAD>(a, ctas, stream);
+  if (j <= 1) return balance_scores<T, 1, 1, SUM, GRAD>(a, ctas, stream);
+  if (j <= 8) return balance_scores<T, 1, 8, SUM, GRAD>(a, ctas, stream);
+  if (j <= 16) return balance_scores<T, 1, 16, SUM, GRAD>(a, ctas, stream);
+  return balance_scores<T, 1, 32, SUM, GRAD>(a, ctas, stream);
 }
 
 template <bool SUM, bool GRAD>
@@ -388,39 +494,62 @@ static int balance_run(const lpmm_b200_balance* b, void* stream_) {
   const int bad = balance_check(b, SUM, GRAD);
   if (bad) return bad;
   cudaStream_t stream = (cudaStream_t)stream_;
-  const BalanceLayout l = balance_layout(b->tokens, b->experts, b->sequences);
-  char* work = reinterpret_cast<char*>(b->work);
   BalanceArgs a = {};
   a.logits = b->logits, a.grad = b->grad, a.index = b->index, a.valid = b->valid, a.offsets = b->offsets;
   a.upstream = b->upstream, a.loss = b->loss, a.factor = b->factor;
   a.counts = reinterpret_cast<unsigned long long*>(b->counts);
+  const BalanceLayout l = balance_layout(b->experts, b->sequences);
   if (SUM) {
-    a.sizes = reinterpret_cast<unsigned long long*>(work);
+    char* work = reinterpret_cast<char*>(b->work);
+    a.psum = reinterpret_cast<unsigned long long*>(work);
+    a.sizes = reinterpret_cast<unsigned long long*>(work + l.sizes_at);
     a.bad = reinterpret_cast<int*>(work + l.bad_at);
-    a.psum = reinterpret_cast<float*>(work + l.psum_at);
-    a.partial = reinterpret_cast<float*>(work + l.partial_at);
+    a.ticket = reinterpret_cast<unsigned*>(work + l.ticket_at);
   }
-  a.tokens = b->tokens, a.inner = b->inner, a.outer_stride = b->outer_stride, a.inner_stride = b->inner_stride;
-  a.sequences = b->sequences, a.tile = l.tile;
-  a.experts = (int)b->experts, a.k = (int)b->k, a.index_bits = b->index_bits, a.offset_bits = b->offset_bits;
+  a.tokens = (int)b->tokens, a.inner = b->inner, a.outer_stride = b->outer_stride, a.inner_stride = b->inner_stride;
+  a.sequences = (int)b->sequences, a.experts = (int)b->experts, a.k = (int)b->k;
+  a.index_bits = b->index_bits, a.offset_bits = b->offset_bits;
   a.sigmoid = b->score == LPMM_B200_SCORE_SIGMOID;
   a.scale = b->grad_scale;
-  if (SUM) {
-    LPMM_CUDA_TRY(cudaMemsetAsync(b->counts, 0, sizeof(int64_t) * b->sequences * b->experts, stream));
-    LPMM_CUDA_TRY(cudaMemsetAsync(work, 0, l.psum_at, stream));
-    balance_count_kernel<<<(unsigned)l.ctas, WARPS * 32, b->sequences == 1 ? sizeof(int) * b->experts : 0, stream>>>(a);
-    LPMM_CUDA_TRY(cudaGetLastError());
+  for (a.shift = 61; a.shift > 1 && (b->tokens >> (62 - a.shift)) != 0;) --a.shift;
+  const int64_t work_size = b->tokens * b->experts;
+  int ctas;
+  const bool wide = balance_wide(b, GRAD);
+  if (SUM && work_size <= SMALL_WORK * SMALL_CLUSTER && b->sequences * b->experts <= 16384 && balance_per_lane(b, wide) <= 8) {
+    ctas = work_size <= SMALL_WORK ? -1 : -SMALL_CLUSTER;
+    a.tile = (int)((b->tokens - ctas - 1) / -ctas);
+  } else {
+    // runs of 8 tokens per warp at least
+    int64_t n = (b->tokens + 63) / 64;
+    if (n > 3 * num_sms()) n = 3 * num_sms();
+    if (n < 1) n = 1;
+    a.tile = (int)((b->tokens + n - 1) / n);
+    ctas = a.tile ? (int)((b->tokens + a.tile - 1) / a.tile) : 1;
+    a.finish = b->sequences <= 64;
   }
-  if (b->tokens) {
+  if (a.tile < 1) a.tile = 1;
+  if (SUM && ctas > 0) {
+    // counts, psum, sizes, bad, ticket: cleared, in one go where the workspace follows the counts
+    const size_t cells = 8 * (size_t)(b->sequences * b->experts);
+    if (reinterpret_cast<char*>(b->counts) + cells == reinterpret_cast<char*>(b->work)) {
+      LPMM_CUDA_TRY(cudaMemsetAsync(b->counts, 0, cells + l.bytes, stream));
+    } else {
+      LPMM_CUDA_TRY(cudaMemsetAsync(b->counts, 0, cells, stream));
+      LPMM_CUDA_TRY(cudaMemsetAsync(b->work, 0, l.bytes, stream));
+    }
+    LPMM_CUDA_TRY(balance_launch(balance_count_kernel, a, ctas, 256, 8 * (size_t)a.experts, 1, false, stream));
+  }
+  if (SUM || b->tokens) {
     if (b->dtype == LPMM_B200_DTYPE_FP32)
-      LPMM_CUDA_TRY((balance_shape<float, SUM, GRAD>(a, l.ctas, stream)));
+      LPMM_CUDA_TRY((balance_shape<float, SUM, GRAD>(a, wide, ctas, stream)));
     else if (b->dtype == LPMM_B200_DTYPE_BF16)
-      LPMM_CUDA_TRY((balance_shape<__nv_bfloat16, SUM, GRAD>(a, l.ctas, stream)));
+      LPMM_CUDA_TRY((balance_shape<__nv_bfloat16, SUM, GRAD>(a, wide, ctas, stream)));
     else
-      LPMM_CUDA_TRY((balance_shape<__half, SUM, GRAD>(a, l.ctas, stream)));
+      LPMM_CUDA_TRY((balance_shape<__half, SUM, GRAD>(a, wide, ctas, stream)));
   }
-  if (SUM) {
-    balance_loss_kernel<<<(unsigned)b->sequences, 256, 0, stream>>>(a);
+  if (SUM && ctas > 0 && !a.finish) {
+    const int64_t n = (b->sequences + 7) / 8;
+    balance_loss_kernel<<<(unsigned)(n < 4096 ? n : 4096), 256, 0, stream>>>(a);
     LPMM_CUDA_TRY(cudaGetLastError());
   }
   return LPMM_B200_OK;
@@ -430,11 +559,10 @@ static int balance_run(const lpmm_b200_balance* b, void* stream_) {
 
 using namespace lpmm_b200;
 
-extern "C" int64_t lpmm_b200_balance_work_bytes(int64_t tokens, int64_t experts, int64_t sequences) {
-  if (tokens < 0 || experts < 1 || sequences < 1 || tokens > (1ll << 40) || experts > LPMM_B200_BALANCE_MAX_EXPERTS ||
-      sequences >= (1ll << 31) - 1)
+extern "C" int64_t lpmm_b200_balance_work_bytes(int64_t experts, int64_t sequences) {
+  if (experts < 1 || sequences < 1 || experts > LPMM_B200_BALANCE_MAX_EXPERTS || sequences > (1 << 24))
     return LPMM_B200_ERR_BAD_SIZE;
-  return balance_layout(tokens, experts, sequences).bytes;
+  return balance_layout(experts, sequences).bytes;
 }
 
 extern "C" int lpmm_b200_balance_forward(const lpmm_b200_balance* b, void* stream) {

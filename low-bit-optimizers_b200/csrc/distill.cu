@@ -146,12 +146,6 @@ struct Expo {
   }
 };
 
-// first element of a row; rows < 2^28, so the division is one of 32 bits
-__device__ __forceinline__ long long row_at(long long row, long long inner, long long outer_stride, long long inner_stride) {
-  if (inner == 1) return row * outer_stride;
-  const unsigned o = (unsigned)row / (unsigned)inner;
-  return o * outer_stride + ((unsigned)row - o * (unsigned)inner) * inner_stride;
-}
 template <typename T>
 __device__ __forceinline__ const T* logits_row(const DistillArgs& a, long long row) {
   return reinterpret_cast<const T*>(a.logits) + row_at(row, a.inner, a.outer_stride, a.inner_stride);
@@ -288,7 +282,7 @@ __device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, 
   t.tm = LOWEST;
   bool any = false, bad = false;
   if (team.rank() == 0) *e.twice = 0;
-#pragma unroll 4
+#pragma unroll(MODE == DISTILL_LOSS ? 2 : 4)
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const long long i = load_index(a.index, row * a.k + k, a.index_bits);
     const float v = load_any(a.teacher, row * a.k + k, a.teacher_dtype);

@@ -124,6 +124,12 @@ __device__ __forceinline__ long long load_index(const void* p, long long i, int 
   return bits == 64 ? reinterpret_cast<const long long*>(p)[i] : (long long)reinterpret_cast<const int*>(p)[i];
 }
 
+// first element of a row; rows and inner < 2^31, so the division is one of 32 bits
+__device__ __forceinline__ long long row_at(long long row, long long inner, long long outer_stride, long long inner_stride) {
+  if (inner == 1) return row * outer_stride;
+  const unsigned o = (unsigned)row / (unsigned)inner;
+  return o * outer_stride + ((unsigned)row - o * (unsigned)inner) * inner_stride;
+}
 // ---------------------------------------------------------------------------------------------
 // barriers in shared memory and bulk copies into it
 // ---------------------------------------------------------------------------------------------

@@ -168,7 +168,7 @@ def _load():
         "lpmm_b200_distill_forward": (i32, [ctypes.POINTER(Distill), vp]),
         "lpmm_b200_distill_backward": (i32, [ctypes.POINTER(Distill), vp]),
         "lpmm_b200_distill_forward_backward": (i32, [ctypes.POINTER(Distill), vp]),
-        "lpmm_b200_balance_work_bytes": (i64, [i64, i64, i64]),
+        "lpmm_b200_balance_work_bytes": (i64, [i64, i64]),
         "lpmm_b200_balance_forward": (i32, [ctypes.POINTER(Balance), vp]),
         "lpmm_b200_balance_backward": (i32, [ctypes.POINTER(Balance), vp]),
         "lpmm_b200_balance_forward_backward": (i32, [ctypes.POINTER(Balance), vp]),

@@ -239,14 +239,20 @@ def _balance_args(router_logits, expert_idx, score, valid, offsets):
 
 
 def _balance_outputs(b, device):
-    """Loss, counts, factor (all ``[sequences, ...]``) and the workspace."""
+    """Loss, counts and factor (``[sequences, ...]``), the workspace behind the counts."""
     s, e = b.sequences, b.experts
-    counts = torch.empty((s, e) if b.offsets else (e,), dtype=torch.int64, device=device)
-    loss = torch.empty((s,) if b.offsets else (), dtype=torch.float32, device=device)
-    factor = torch.empty(s, dtype=torch.float32, device=device)
-    work = torch.empty(N.lib.lpmm_b200_balance_work_bytes(b.tokens, e, s), dtype=torch.uint8, device=device)
-    b.counts, b.loss, b.factor, b.work = counts.data_ptr(), loss.data_ptr(), factor.data_ptr(), work.data_ptr()
-    return loss, counts, factor, work
+    cells = s * e
+    # psum [s, e], sizes [s], flags 4 (s + 1), ticket 4: lpmm_b200_balance_work_bytes, which refuses what is too large
+    nbytes = N.lib.lpmm_b200_balance_work_bytes(e, s)
+    if nbytes < 0:
+        N.check(int(nbytes))
+    buf = torch.empty(cells + nbytes // 8, dtype=torch.int64, device=device)
+    counts = buf[:cells].view(s, e) if b.offsets else buf[:cells]
+    out = torch.empty(2 * s, dtype=torch.float32, device=device)
+    loss, factor = (out[:s] if b.offsets else out[0]), out[s:]
+    b.counts, b.loss = counts.data_ptr(), out.data_ptr()
+    b.factor, b.work = b.loss + 4 * s, b.counts + 8 * cells
+    return loss, counts, factor, buf
 
 
 class _BalanceLoss(torch.autograd.Function):

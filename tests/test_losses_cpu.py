@@ -179,8 +179,8 @@ def test_structures_as_the_library_gets_them(host):
 def test_library_refuses_bad_arguments_before_any_launch():
     lib, ref = N.lib, ctypes.byref
     assert lib.lpmm_b200_distill_work_floats(3) == 19 and lib.lpmm_b200_distill_work_floats(-1) == -2
-    assert lib.lpmm_b200_balance_work_bytes(-1, 8, 1) == -2 and lib.lpmm_b200_balance_work_bytes(4, 1025, 1) == -2
-    assert lib.lpmm_b200_balance_work_bytes(0, 1, 1) > 0
+    assert lib.lpmm_b200_balance_work_bytes(0, 1) == -2 and lib.lpmm_b200_balance_work_bytes(1025, 1) == -2
+    assert lib.lpmm_b200_balance_work_bytes(1, 1) > 0
     forms = (lib.lpmm_b200_distill_forward, lib.lpmm_b200_distill_backward, lib.lpmm_b200_distill_forward_backward)
     good = dict(rows=1, inner=1, outer_stride=8, vocab=8, k=1, index_bits=32, temperature=1.0, grad_scale=1.0)
     for fn in forms:
@@ -208,5 +208,5 @@ def test_library_refuses_bad_arguments_before_any_launch():
         for change, status in ((dict(tokens=-1), -2), (dict(inner=0), -2), (dict(experts=0), -2), (dict(k=0), -2),
                                (dict(sequences=0), -2), (dict(sequences=2), -3), (dict(dtype=7), -3), (dict(index_bits=8), -3),
                                (dict(score=2), -3), (dict(offsets=at, offset_bits=0), -3), (dict(experts=1025), -6),
-                               (dict(k=1025), -6), (dict(), -1)):
+                               (dict(k=1025), -6), (dict(tokens=(1 << 30) + 1), -6), (dict(), -1)):
             assert fn(ref(N.Balance(**dict(good, **change))), None) == status, (fn.__name__, change)
