@@ -45,8 +45,21 @@ __device__ __forceinline__ long long raw_offset(const BalanceArgs& a, int i) {
   if (!a.offsets) return i == 0 ? 0 : a.tokens;
   return load_index(a.offsets, i, a.offset_bits);
 }
-__device__ __forceinline__ int offset_at(const BalanceArgs& a, int i) {
+// Offsets kept within [0, tokens], in shared memory where there are few: a search is then a matter of nanoseconds.
+constexpr int SHARED_OFFSETS = 1024;
+struct Offsets {
+  int at[SHARED_OFFSETS + 1];
+};
+__device__ __forceinline__ int clamped_offset(const BalanceArgs& a, int i) {
   return (int)min(max(raw_offset(a, i), 0ll), (long long)a.tokens);
+}
+__device__ __forceinline__ void load_offsets(const BalanceArgs& a, Offsets& o) {
+  if (a.offsets && a.sequences <= SHARED_OFFSETS)
+    for (int i = threadIdx.x; i <= a.sequences; i += blockDim.x) o.at[i] = clamped_offset(a, i);
+  __syncthreads();
+}
+__device__ __forceinline__ int offset_at(const BalanceArgs& a, const Offsets& o, int i) {
+  return a.sequences <= SHARED_OFFSETS ? o.at[i] : clamped_offset(a, i);
 }
 
 // The stretch of tokens from r on that belongs to one sequence: s in [0, sequences), or s < 0 for tokens of none.
@@ -54,26 +67,27 @@ __device__ __forceinline__ int offset_at(const BalanceArgs& a, int i) {
 struct Stretch {
   int s, end;
 };
-__device__ __forceinline__ Stretch stretch_at(const BalanceArgs& a, int r, int hi) {
+__device__ __forceinline__ Stretch stretch_at(const BalanceArgs& a, const Offsets& o, int r, int hi) {
   if (!a.offsets) return Stretch{0, hi};
   int lo = -1, up = a.sequences + 1;  // offset(lo) <= r < offset(up)
   while (up - lo > 1) {
     const int mid = (lo + up) >> 1;
-    if (offset_at(a, mid) <= r)
+    if (offset_at(a, o, mid) <= r)
       lo = mid;
     else
       up = mid;
   }
   if (lo == a.sequences) return Stretch{-1, hi};
-  return Stretch{lo, max(min(offset_at(a, lo + 1), hi), r + 1)};
+  return Stretch{lo, max(min(offset_at(a, o, lo + 1), hi), r + 1)};
 }
 
 __device__ __forceinline__ long long cell(const BalanceArgs& a, int s, int e) { return (long long)s * a.experts + e; }
 
 // (what earlier phases of the same launch have written is read past L1)
 __device__ __forceinline__ double factor_of(const BalanceArgs& a, int s) {
-  if ((__ldcg(&a.bad[s]) & 1) || __ldcg(&a.bad[a.sequences])) return (double)nan_f();
+  const int bad = __ldcg(&a.bad[s]), off = __ldcg(&a.bad[a.sequences]);
   const double n = (double)__ldcg(&a.sizes[s]);
+  if ((bad & 1) | off) return (double)nan_f();
   return n == 0.0 ? 0.0 : (double)a.experts / ((double)a.k * n * n);
 }
 
@@ -81,13 +95,13 @@ __device__ __forceinline__ double factor_of(const BalanceArgs& a, int s) {
 // have many tokens here); sequences between them lie within the CTA and go straight to memory.
 struct Tile {
   int lo, hi, first, last;
-  __device__ __forceinline__ Tile(const BalanceArgs& a, int cta) {
+  __device__ __forceinline__ Tile(const BalanceArgs& a, const Offsets& o, int cta) {
     lo = (int)min((long long)cta * a.tile, (long long)a.tokens);
     hi = min(lo + a.tile, a.tokens);
     first = last = -1;
     if (lo < hi) {
-      first = stretch_at(a, lo, hi).s;
-      last = stretch_at(a, hi - 1, hi).s;
+      first = stretch_at(a, o, lo, hi).s;
+      last = stretch_at(a, o, hi - 1, hi).s;
     }
   }
   // this warp's run
@@ -100,23 +114,23 @@ struct Tile {
 };
 
 // Assignments per expert and valid tokens per sequence.  hist: int[2, experts] in shared memory
-__device__ __forceinline__ void count_phase(const BalanceArgs& a, int cta, int* hist) {
+__device__ __forceinline__ void count_phase(const BalanceArgs& a, const Offsets& o, int cta, int* hist) {
   const int lane = threadIdx.x & 31;
   if (cta == 0 && a.offsets) {
     bool off = false;
     for (int i = threadIdx.x; i <= a.sequences; i += blockDim.x) {
-      const long long o = raw_offset(a, i);
-      off |= o < 0 || o > a.tokens || (i && raw_offset(a, i - 1) > o);
+      const long long at = raw_offset(a, i);
+      off |= at < 0 || at > a.tokens || (i && raw_offset(a, i - 1) > at);
     }
     if (off) a.bad[a.sequences] = 1;
   }
   for (int e = threadIdx.x; e < 2 * a.experts; e += blockDim.x) hist[e] = 0;
-  const Tile tile(a, cta);
+  const Tile tile(a, o, cta);
   __syncthreads();
   int lo, hi;
   tile.run(lo, hi);
   for (int r = lo; r < hi;) {
-    const Stretch t = stretch_at(a, r, hi);
+    const Stretch t = stretch_at(a, o, r, hi);
     if (t.s >= 0) {
       const int set = tile.set(t.s);
       int size = 0;
@@ -154,92 +168,153 @@ __device__ __forceinline__ void count_phase(const BalanceArgs& a, int cta, int* 
   }
 }
 
+// Logits as they lie in memory, for U tokens per group of lanes
+template <typename T, int V, int J, int U>
+struct Raw {
+  static constexpr int WORDS = V == 1 ? 1 : 4;
+  uint32_t w[U][J][WORDS];
+  bool ok[U];
+  // tokens base + u * per + gi below `end`; what is not there, or not valid, is 0, a column that is not there -inf
+  __device__ __forceinline__ void load(const BalanceArgs& a, int base, int end, bool any, int per, int gi, int gl) {
+    using E = Elem<T>;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int r = base + u * per + gi;
+      ok[u] = any && r < end && (!a.valid || a.valid[r]);
+      const T* row = reinterpret_cast<const T*>(a.logits) + row_at(r, a.inner, a.outer_stride, a.inner_stride);
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const int col = (j * a.group + gl) * V;
+        const uint32_t fill = ok[u] ? E::none().x : 0u;
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) w[u][j][i] = fill;
+        if (ok[u] && col < a.experts) {
+          if constexpr (V == 1) {
+            w[u][j][0] = E::raw(row + col);
+          } else {
+            const uint4 q = *reinterpret_cast<const uint4*>(row + col);
+            w[u][j][0] = q.x, w[u][j][1] = q.y, w[u][j][2] = q.z, w[u][j][3] = q.w;
+          }
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void unpack(int u, float* x) const {
+    using E = Elem<T>;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      if constexpr (V == 1)
+        x[j] = E::of_raw(w[u][j][0]);
+      else
+        E::unpack(make_uint4(w[u][j][0], w[u][j][1], w[u][j][2], w[u][j][3]), x + j * V);
+    }
+  }
+};
+
 // Scores of all tokens: their sums (SUM), the gradient (GRAD).  V: elements per load (16 bytes, or 1 where rows are
 // not 16-byte aligned), J: loads per lane; a.group lanes (a power of two) hold a token's logits, U tokens each are under
-// way at a time.  sums: unsigned long long[2, experts] in shared memory
-template <typename T, int V, int J, bool SIG, bool SUM, bool GRAD>
-__device__ __forceinline__ void score_phase(const BalanceArgs& a, int cta, unsigned long long* sums) {
+// way at a time and the next U on their way from memory.  sums: unsigned long long[2, experts] in shared memory, behind them
+// float[2, experts]: the counts of the CTA's first and last sequence (read once per CTA: thousands of warps that read the
+// same few lines of L2 wait for one another, 10 us at 256 experts)
+template <typename T, int V, int J, int U, bool SIG, bool SUM, bool GRAD>
+__device__ __forceinline__ void score_phase(const BalanceArgs& a, const Offsets& o, int cta, unsigned long long* sums) {
   using E = Elem<T>;
-  constexpr int U = J * V <= 8 ? (SIG ? 2 : 4) : J * V <= 16 && !SIG ? 2 : 1;
+  constexpr int JV = J * V, N2 = (JV + 1) / 2;  // pairs; an odd last one is filled up with -inf
   const int lane = threadIdx.x & 31;
   const int G = a.group, per = 32 / G, gl = lane & (G - 1), gi = lane / G;
   if (SUM)
     for (int e = threadIdx.x; e < 2 * a.experts; e += blockDim.x) sums[e] = 0;
-  const Tile tile(a, cta);
-  if (SUM) __syncthreads();
+  const Tile tile(a, o, cta);
+  float* counts = reinterpret_cast<float*>(SUM ? sums + 2 * a.experts : sums);
+  if (GRAD) {
+    if (SUM) pdl_wait();  // the counts
+    for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
+      if (tile.first >= 0) counts[e] = (float)__ldcg(&a.counts[cell(a, tile.first, e)]);
+      if (tile.last >= 0) counts[a.experts + e] = (float)__ldcg(&a.counts[cell(a, tile.last, e)]);
+    }
+  }
+  __syncthreads();
   int lo, hi;
   tile.run(lo, hi);
   constexpr float LOG2E = 1.4426950408889634f;
   const float minus_inf = -__int_as_float(0x7f800000), units = __int_as_float((a.shift + 127) << 23);
+  const f2 log2e = f2_splat(LOG2E), zero = f2_splat(0.0f);
 
   for (int r0 = lo; r0 < hi;) {
-    const Stretch t = stretch_at(a, r0, hi);
-    float c[J * V], acc[J * V], fac = 0.0f;
-    if (GRAD && t.s >= 0) {
-      fac = a.scale * (SUM ? (float)factor_of(a, t.s) : a.factor[t.s] * a.upstream[t.s]);
+    const Stretch t = stretch_at(a, o, r0, hi);
+    const bool any = t.s >= 0;
+    Raw<T, V, J, U> next;
+    next.load(a, r0, t.end, any, per, gi, gl);
+    f2 c[N2], acc[N2];
+    float fac = 0.0f;
+    const int set = tile.set(t.s);
+    if (GRAD && any) fac = a.scale * (SUM ? (float)factor_of(a, t.s) : a.factor[t.s] * a.upstream[t.s]);
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+    for (int n = 0; n < N2; ++n) {
+      float v[2] = {0.0f, 0.0f};
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const int col = (j * G + gl) * V + i;
-          c[j * V + i] = col < a.experts ? (float)__ldcg(&a.counts[cell(a, t.s, col)]) : 0.0f;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < J * V; ++i) acc[i] = 0.0f;
-    for (int base = r0; base < t.end; base += per * U) {
-      bool here[U], ok[U];
-      float x[U][J * V], m[U], sum[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = base + u * per + gi;
-        here[u] = r < t.end;
-        ok[u] = here[u] && t.s >= 0 && (!a.valid || a.valid[r]);
-        const T* row = reinterpret_cast<const T*>(a.logits) + row_at(r, a.inner, a.outer_stride, a.inner_stride);
-#pragma unroll
-        for (int j = 0; j < J; ++j) {
-          const int col = (j * G + gl) * V;
-          const bool in = ok[u] && col < a.experts;
-          if constexpr (V == 1) {
-            x[u][j] = in ? E::widen(row[col]) : ok[u] ? minus_inf : 0.0f;
-          } else {
-            const uint4 w = in ? *reinterpret_cast<const uint4*>(row + col) : ok[u] ? E::none() : make_uint4(0, 0, 0, 0);
-            E::unpack(w, x[u] + j * V);
-          }
-        }
+      for (int h = 0; h < 2; ++h) {
+        const int i = 2 * n + h, col = (i / V * G + gl) * V + i % V;
+        if (GRAD && any && i < JV && col < a.experts)
+          v[h] = set >= 0 ? counts[set * a.experts + col] : (float)__ldcg(&a.counts[cell(a, t.s, col)]);
       }
+      c[n] = f2_pack(v[0], v[1]);
+      acc[n] = zero;
+    }
+    for (int base = r0; base < t.end; base += per * U) {
+      const Raw<T, V, J, U> now = next;
+      if (base + per * U < t.end) next.load(a, base + per * U, t.end, any, per, gi, gl);
+      f2 p[U][N2];                 // the scores
+      f2 slope[SIG ? U : 1][N2];   // 1 - sigmoid
+      float m[U], sum[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        m[u] = x[u][0];
+        float x[2 * N2];
+        x[2 * N2 - 1] = minus_inf;
+        now.unpack(u, x);
+        m[u] = x[0];
 #pragma unroll
-        for (int i = 1; i < J * V; ++i) m[u] = fmaxf(m[u], x[u][i]);
+        for (int i = 1; i < JV; ++i) m[u] = fmaxf(m[u], x[i]);
+#pragma unroll
+        for (int n = 0; n < N2; ++n) p[u][n] = f2_pack(x[2 * n], x[2 * n + 1]);
       }
       for (int d = G >> 1; d; d >>= 1) {
 #pragma unroll
         for (int u = 0; u < U; ++u) m[u] = fmaxf(m[u], __shfl_xor_sync(~0u, m[u], d));
       }
-      // p: the score; x (sigmoid only): 1 - sigmoid
-      float p[U][J * V];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        sum[u] = 0.0f;
+        f2 total = zero;
         if constexpr (SIG) {
           // sigmoid(x) = e^min(x,0) / (1 + e^-|x|), scaled by e^-min(m,0) so that the largest one stays near 1
           const float top = fminf(m[u], 0.0f);
 #pragma unroll
-          for (int i = 0; i < J * V; ++i) {
-            const float v = x[u][i], fall = ex2(-fabsf(v) * LOG2E), d = rcp_nr(1.0f + fall);
-            p[u][i] = v == v ? ex2((fminf(v, 0.0f) - top) * LOG2E) * d : v;
-            x[u][i] = v >= 0.0f ? fall * d : d;
-            sum[u] += p[u][i];
+          for (int n = 0; n < N2; ++n) {
+            float x[2], y[2], z[2];
+            f2_unpack(p[u][n], x[0], x[1]);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float v = x[h], fall = ex2(-fabsf(v) * LOG2E), d = rcp_nr(1.0f + fall);
+              y[h] = v == v ? ex2((fminf(v, 0.0f) - top) * LOG2E) * d : v;
+              z[h] = v >= 0.0f ? fall * d : d;
+            }
+            p[u][n] = f2_pack(y[0], y[1]);
+            slope[u][n] = f2_pack(z[0], z[1]);
+            total = f2_add(total, p[u][n]);
           }
         } else {
+          const f2 top = f2_splat(-m[u]);
 #pragma unroll
-          for (int i = 0; i < J * V; ++i) {
-            p[u][i] = ex2((x[u][i] - m[u]) * LOG2E);
-            sum[u] += p[u][i];
+          for (int n = 0; n < N2; ++n) {
+            float x, y;
+            f2_unpack(f2_mul(f2_add(p[u][n], top), log2e), x, y);
+            p[u][n] = f2_pack(ex2(x), ex2(y));
+            total = f2_add(total, p[u][n]);
           }
         }
+        float x, y;
+        f2_unpack(total, x, y);
+        sum[u] = x + y;
       }
       for (int d = G >> 1; d; d >>= 1) {
 #pragma unroll
@@ -248,14 +323,17 @@ __device__ __forceinline__ void score_phase(const BalanceArgs& a, int cta, unsig
       float dot[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const float inv = rcp_nr(sum[u]);
-        dot[u] = 0.0f;
+        const f2 inv = f2_splat(now.ok[u] ? rcp_nr(sum[u]) : 0.0f);  // 0: the logits stand as 0, the scores are 0 from here on
+        f2 total = zero;
 #pragma unroll
-        for (int i = 0; i < J * V; ++i) {
-          p[u][i] *= inv;
-          if (SUM) acc[i] += ok[u] ? p[u][i] : 0.0f;
-          if (GRAD) dot[u] = fmaf(c[i], p[u][i], dot[u]);
+        for (int n = 0; n < N2; ++n) {
+          p[u][n] = f2_mul(p[u][n], inv);
+          if (SUM) acc[n] = f2_add(acc[n], p[u][n]);
+          if (GRAD) total = f2_fma(c[n], p[u][n], total);
         }
+        float x, y;
+        f2_unpack(total, x, y);
+        dot[u] = x + y;
       }
       if (GRAD) {
         for (int d = G >> 1; d; d >>= 1) {
@@ -264,46 +342,49 @@ __device__ __forceinline__ void score_phase(const BalanceArgs& a, int cta, unsig
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-          T* g = reinterpret_cast<T*>(a.grad) + (long long)(base + u * per + gi) * a.experts;
+          const int r = base + u * per + gi;
+          const f2 f = f2_splat(now.ok[u] ? fac : 0.0f), less = f2_splat(-dot[u]);
+          float y[2 * N2];
+#pragma unroll
+          for (int n = 0; n < N2; ++n) {
+            f2 v = f2_mul(f2_mul(f, p[u][n]), f2_add(c[n], less));
+            if (SIG) v = f2_mul(v, slope[SIG ? u : 0][n]);
+            f2_unpack(v, y[2 * n], y[2 * n + 1]);
+          }
+          T* g = reinterpret_cast<T*>(a.grad) + (long long)r * a.experts;
 #pragma unroll
           for (int j = 0; j < J; ++j) {
             const int col = (j * G + gl) * V;
-            float y[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              float v = fac * p[u][j * V + i] * (c[j * V + i] - dot[u]);
-              if (SIG) v *= x[u][j * V + i];
-              y[i] = ok[u] ? v : 0.0f;
-            }
-            if (here[u] && col < a.experts) {
+            if (r < t.end && col < a.experts) {
               if constexpr (V == 1)
-                g[col] = E::narrow(y[0]);
+                g[col] = E::narrow(y[j]);
               else
-                *reinterpret_cast<uint4*>(g + col) = E::pack(y);
+                *reinterpret_cast<uint4*>(g + col) = E::pack(y + j * V);
             }
           }
         }
       }
     }
-    if (SUM && t.s >= 0) {
-      const int set = tile.set(t.s);
+    if (SUM && any) {
       bool nan = false;
 #pragma unroll
-      for (int j = 0; j < J; ++j)
+      for (int n = 0; n < N2; ++n) {
+        float v[2];
+        f2_unpack(acc[n], v[0], v[1]);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          float v = acc[j * V + i];
-          for (int d = G; d < 32; d <<= 1) v += __shfl_xor_sync(~0u, v, d);
-          const int col = (j * G + gl) * V + i;
-          if (gi == 0 && col < a.experts) {
-            nan |= !(v == v);
-            const unsigned long long n = (unsigned long long)__float2ll_rn(v * units);
+        for (int h = 0; h < 2; ++h) {
+          const int i = 2 * n + h, col = (i / V * G + gl) * V + i % V;
+          for (int d = G; d < 32; d <<= 1) v[h] += __shfl_xor_sync(~0u, v[h], d);
+          if (gi == 0 && i < JV && col < a.experts) {
+            nan |= !(v[h] == v[h]);
+            const unsigned long long q = (unsigned long long)__float2ll_rn(v[h] * units);
             if (set >= 0)
-              atomicAdd(&sums[set * a.experts + col], n);
+              atomicAdd(&sums[set * a.experts + col], q);
             else
-              atomicAdd(&a.psum[cell(a, t.s, col)], n);
+              atomicAdd(&a.psum[cell(a, t.s, col)], q);
           }
         }
+      }
       if (nan) atomicOr(&a.bad[t.s], 2);
     }
     r0 = t.end;
@@ -316,35 +397,57 @@ __device__ __forceinline__ void score_phase(const BalanceArgs& a, int cta, unsig
   }
 }
 
-// Loss and factor of the sequences s = first, first + step, ...: one warp each.  Reads what other CTAs have written.
-__device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int step) {
-  const int lane = threadIdx.x & 31;
-  for (int s = first; s < a.sequences; s += step) {
-    double sum = 0.0;
-    for (int e = lane; e < a.experts; e += 32)
-      sum += (double)__ldcg(&a.counts[cell(a, s, e)]) * (double)__ldcg(&a.psum[cell(a, s, e)]);
+__device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(~0u, sum, d);
+  for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+  return v;
+}
+
+// Loss and factor of the sequences.  Reads what other CTAs have written; the loads of a thread are independent of one
+// another.  A sequence has a warp, or, where there is one sequence only, the CTA (`red`: double[32]).
+__device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int step, double* red) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool one = a.sequences == 1;
+  for (int s = one ? 0 : first + warp; s < a.sequences; s += step) {
+    double sum = 0.0;
+    const int from = one ? threadIdx.x : lane, by = one ? blockDim.x : 32;
+#pragma unroll 4
+    for (int e = from; e < a.experts; e += by)
+      sum += (double)__ldcg(&a.counts[cell(a, s, e)]) * (double)__ldcg(&a.psum[cell(a, s, e)]);
+    const double f = factor_of(a, s);
+    const int nan = __ldcg(&a.bad[s]) & 2;
+    sum = warp_sum(sum);
+    if (one) {
+      if (lane == 0) red[warp] = sum;
+      __syncthreads();
+      sum = warp_sum(lane < (int)(blockDim.x >> 5) ? red[lane] : 0.0);
+      if (warp != 0) return;
+    }
     if (lane == 0) {
-      const double f = factor_of(a, s);
       a.factor[s] = (float)f;
-      a.loss[s] = __ldcg(&a.bad[s]) & 2 ? nan_f() : (float)(sum * f * exp2(-(double)a.shift));
+      a.loss[s] = nan ? nan_f() : (float)(sum * f * __longlong_as_double((1023ll - a.shift) << 52));
     }
   }
 }
 
-__global__ void __launch_bounds__(256) balance_count_kernel(const BalanceArgs a) {
+__global__ void __launch_bounds__(1024) balance_count_kernel(const BalanceArgs a) {
   extern __shared__ unsigned long long shared[];
+  __shared__ Offsets offsets;
   pdl_start_next();
-  count_phase(a, blockIdx.x, reinterpret_cast<int*>(shared));
+  load_offsets(a, offsets);
+  count_phase(a, offsets, blockIdx.x, reinterpret_cast<int*>(shared));
 }
 
 template <typename T, int V, int J, bool SIG, bool SUM, bool GRAD>
-__global__ void __launch_bounds__(256, J * V <= 8 ? 3 : 2) balance_score_kernel(const BalanceArgs a) {
+__global__ void __launch_bounds__(256, 2) balance_score_kernel(const BalanceArgs a) {
   extern __shared__ unsigned long long shared[];
+  __shared__ Offsets offsets;
   __shared__ bool last;
-  pdl_wait();
-  score_phase<T, V, J, SIG, SUM, GRAD>(a, blockIdx.x, shared);
+  __shared__ double red[32];
+  constexpr int U = J * V <= 8 ? (SIG ? 2 : 4) : J * V <= 16 && !SIG ? 2 : 1;
+  load_offsets(a, offsets);
+  score_phase<T, V, J, U, SIG, SUM, GRAD>(a, offsets, blockIdx.x, shared);
+  if (SUM) pdl_wait();  // without the gradient nothing needs the counts but the CTA that adds up
   if (SUM && a.finish) {
     __threadfence();
     __syncthreads();
@@ -352,19 +455,22 @@ __global__ void __launch_bounds__(256, J * V <= 8 ? 3 : 2) balance_score_kernel(
     __syncthreads();
     if (last) {
       __threadfence();
-      loss_phase(a, threadIdx.x >> 5, blockDim.x >> 5);
+      loss_phase(a, 0, blockDim.x >> 5, red);
     }
   }
 }
 
 __global__ void __launch_bounds__(256) balance_loss_kernel(const BalanceArgs a) {
-  loss_phase(a, (blockIdx.x * blockDim.x + threadIdx.x) >> 5, gridDim.x * (blockDim.x >> 5));
+  __shared__ double red[32];
+  loss_phase(a, blockIdx.x * (blockDim.x >> 5), gridDim.x * (blockDim.x >> 5), red);
 }
 
 // Everything in one launch of one cluster (of one CTA, where that is enough).
-template <typename T, int V, int J, bool SIG, bool GRAD>
+template <typename T, int V, int J, int U, bool SIG, bool GRAD>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 1) balance_small_kernel(const BalanceArgs a) {
   extern __shared__ unsigned long long shared[];
+  __shared__ Offsets offsets;
+  __shared__ double red[32];
   cg::cluster_group cluster = cg::this_cluster();
   const int ctas = gridDim.x, cta = blockIdx.x;
   const auto all = [&] {
@@ -380,13 +486,19 @@ __global__ void __launch_bounds__(MAX_WARPS * 32, 1) balance_small_kernel(const 
     if (i < a.sequences) a.sizes[i] = 0;
     a.bad[i] = 0;
   }
+  load_offsets(a, offsets);
   all();
-  count_phase(a, cta, reinterpret_cast<int*>(shared));
+  count_phase(a, offsets, cta, reinterpret_cast<int*>(shared));
   all();
-  score_phase<T, V, J, SIG, true, GRAD>(a, cta, shared);
+  score_phase<T, V, J, U, SIG, true, GRAD>(a, offsets, cta, shared);
   all();
-  loss_phase(a, (int)(id >> 5), ctas * (blockDim.x >> 5));
+  if (a.sequences > 1 || cta == 0) loss_phase(a, cta * (blockDim.x >> 5), ctas * (blockDim.x >> 5), red);
 }
+
+constexpr int BALANCE_CTAS = 2;  // per SM, all at once
+constexpr int COUNT_CTAS = 74;   // of 1024 threads: few, for their atomics on the counts follow one another
+constexpr int SMALL_CLUSTER = 8;
+constexpr int64_t SMALL_WORK = 8192, MEDIUM_WORK = 262144;  // logits for one CTA, for one cluster
 
 // workspace: psum, sizes, bad, ticket
 struct BalanceLayout {
@@ -441,18 +553,18 @@ static cudaError_t balance_launch(K kernel, const BalanceArgs& a, int ctas, int 
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-constexpr int SMALL_CLUSTER = 8;
-constexpr int64_t SMALL_WORK = 32768;  // logits per CTA up to which one launch is quicker than three
-
 // ctas < 0: everything in one launch of a cluster of -ctas
 template <typename T, int V, int J, bool SUM, bool GRAD>
 static cudaError_t balance_scores(const BalanceArgs& a, int ctas, cudaStream_t stream) {
-  const size_t smem = SUM ? 16 * (size_t)a.experts : 0;
+  const size_t smem = (SUM ? 16 : 0) * (size_t)a.experts + (GRAD ? 8 : 0) * (size_t)a.experts;
   if constexpr (SUM && J * V <= 8) {
+    if (ctas == -1)  // one token at a time: less code to fetch
+      return a.sigmoid ? balance_launch(balance_small_kernel<T, V, J, 1, true, GRAD>, a, 1, MAX_WARPS * 32, smem, 1, false, stream)
+                       : balance_launch(balance_small_kernel<T, V, J, 1, false, GRAD>, a, 1, MAX_WARPS * 32, smem, 1, false, stream);
     if (ctas < 0)
       return a.sigmoid
-                 ? balance_launch(balance_small_kernel<T, V, J, true, GRAD>, a, -ctas, MAX_WARPS * 32, smem, -ctas, false, stream)
-                 : balance_launch(balance_small_kernel<T, V, J, false, GRAD>, a, -ctas, MAX_WARPS * 32, smem, -ctas, false, stream);
+                 ? balance_launch(balance_small_kernel<T, V, J, 2, true, GRAD>, a, -ctas, MAX_WARPS * 32, smem, -ctas, false, stream)
+                 : balance_launch(balance_small_kernel<T, V, J, 4, false, GRAD>, a, -ctas, MAX_WARPS * 32, smem, -ctas, false, stream);
   }
   return a.sigmoid ? balance_launch(balance_score_kernel<T, V, J, true, SUM, GRAD>, a, ctas, 256, smem, 1, SUM, stream)
                    : balance_launch(balance_score_kernel<T, V, J, false, SUM, GRAD>, a, ctas, 256, smem, 1, SUM, stream);
@@ -515,13 +627,13 @@ static int balance_run(const lpmm_b200_balance* b, void* stream_) {
   const int64_t work_size = b->tokens * b->experts;
   int ctas;
   const bool wide = balance_wide(b, GRAD);
-  if (SUM && work_size <= SMALL_WORK * SMALL_CLUSTER && b->sequences * b->experts <= 16384 && balance_per_lane(b, wide) <= 8) {
+  if (SUM && work_size <= MEDIUM_WORK && b->sequences * b->experts <= 16384 && balance_per_lane(b, wide) <= 8) {
     ctas = work_size <= SMALL_WORK ? -1 : -SMALL_CLUSTER;
     a.tile = (int)((b->tokens - ctas - 1) / -ctas);
   } else {
     // runs of 8 tokens per warp at least
     int64_t n = (b->tokens + 63) / 64;
-    if (n > 3 * num_sms()) n = 3 * num_sms();
+    if (n > BALANCE_CTAS * num_sms()) n = BALANCE_CTAS * num_sms();
     if (n < 1) n = 1;
     a.tile = (int)((b->tokens + n - 1) / n);
     ctas = a.tile ? (int)((b->tokens + a.tile - 1) / a.tile) : 1;
@@ -537,7 +649,12 @@ static int balance_run(const lpmm_b200_balance* b, void* stream_) {
       LPMM_CUDA_TRY(cudaMemsetAsync(b->counts, 0, cells, stream));
       LPMM_CUDA_TRY(cudaMemsetAsync(b->work, 0, l.bytes, stream));
     }
-    LPMM_CUDA_TRY(balance_launch(balance_count_kernel, a, ctas, 256, 8 * (size_t)a.experts, 1, false, stream));
+    BalanceArgs c = a;
+    int n = (int)((b->tokens + 255) / 256);
+    if (n > COUNT_CTAS) n = COUNT_CTAS;
+    if (n < 1) n = 1;
+    c.tile = (int)((b->tokens + n - 1) / n);
+    LPMM_CUDA_TRY(balance_launch(balance_count_kernel, c, n, 1024, 8 * (size_t)a.experts, 1, false, stream));
   }
   if (SUM || b->tokens) {
     if (b->dtype == LPMM_B200_DTYPE_FP32)

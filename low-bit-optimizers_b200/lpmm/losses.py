@@ -239,31 +239,29 @@ def _balance_args(router_logits, expert_idx, score, valid, offsets):
 
 
 def _balance_outputs(b, device):
-    """Loss, counts and factor (``[sequences, ...]``), the workspace behind the counts."""
+    """Loss, counts, and the buffer that holds the counts, the workspace behind them and the gradient's factors."""
     s, e = b.sequences, b.experts
     cells = s * e
-    # psum [s, e], sizes [s], flags 4 (s + 1), ticket 4: lpmm_b200_balance_work_bytes, which refuses what is too large
-    nbytes = N.lib.lpmm_b200_balance_work_bytes(e, s)
+    nbytes = N.lib.lpmm_b200_balance_work_bytes(e, s)  # a multiple of 16
     if nbytes < 0:
         N.check(int(nbytes))
-    buf = torch.empty(cells + nbytes // 8, dtype=torch.int64, device=device)
-    counts = buf[:cells].view(s, e) if b.offsets else buf[:cells]
-    out = torch.empty(2 * s, dtype=torch.float32, device=device)
-    loss, factor = (out[:s] if b.offsets else out[0]), out[s:]
-    b.counts, b.loss = counts.data_ptr(), out.data_ptr()
-    b.factor, b.work = b.loss + 4 * s, b.counts + 8 * cells
-    return loss, counts, factor, buf
+    buf = torch.empty(cells + nbytes // 8 + (s + 1) // 2, dtype=torch.int64, device=device)
+    loss = torch.empty((s,) if b.offsets else (), dtype=torch.float32, device=device)
+    at = buf.data_ptr()
+    b.counts, b.work, b.factor, b.loss = at, at + 8 * cells, at + 8 * cells + nbytes, loss.data_ptr()
+    counts = buf[:cells]
+    return loss, counts.view(s, e) if b.offsets else counts, buf
 
 
 class _BalanceLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, router_logits, expert_idx, score, valid, offsets):
         b, kept = _balance_args(router_logits, expert_idx, score, valid, offsets)
-        loss, counts, factor, work = _balance_outputs(b, router_logits.device)
+        loss, counts, ctx.buf = _balance_outputs(b, router_logits.device)
         _launch(N.lib.lpmm_b200_balance_forward, b, router_logits.device)
         ctx.mark_non_differentiable(counts)
         ctx.save_for_backward(router_logits, expert_idx, valid, offsets, counts)
-        ctx.factor, ctx.score = factor, score
+        ctx.factor, ctx.score = b.factor, score
         return loss, counts
 
     @staticmethod
@@ -273,7 +271,7 @@ class _BalanceLoss(torch.autograd.Function):
         b, kept = _balance_args(router_logits, expert_idx, ctx.score, valid, offsets)
         grad = torch.empty(router_logits.shape, dtype=router_logits.dtype, device=router_logits.device)
         upstream = upstream.to(torch.float32).contiguous()
-        b.grad, b.upstream, b.counts, b.factor = grad.data_ptr(), upstream.data_ptr(), counts.data_ptr(), ctx.factor.data_ptr()
+        b.grad, b.upstream, b.counts, b.factor = grad.data_ptr(), upstream.data_ptr(), counts.data_ptr(), ctx.factor
         _launch(N.lib.lpmm_b200_balance_backward, b, router_logits.device)
         return grad, None, None, None, None
 
@@ -298,7 +296,7 @@ def balance_loss(router_logits, expert_idx, score="softmax", valid=None, offsets
     if torch.is_grad_enabled() and isinstance(router_logits, torch.Tensor) and router_logits.requires_grad:
         return _BalanceLoss.apply(router_logits, expert_idx, score, valid, offsets)
     b, kept = _balance_args(router_logits, expert_idx, score, valid, offsets)
-    loss, counts, factor, work = _balance_outputs(b, router_logits.device)
+    loss, counts, buf = _balance_outputs(b, router_logits.device)
     _launch(N.lib.lpmm_b200_balance_forward, b, router_logits.device)
     return loss, counts
 
@@ -309,7 +307,7 @@ def balance_loss_with_grad(router_logits, expert_idx, score="softmax", valid=Non
     ``grad`` is ``grad_scale`` times the derivative of the loss (of the losses' sum with ``offsets``) by
     ``router_logits``: a new contiguous tensor of their shape and type.  Nothing takes part in autograd."""
     b, kept = _balance_args(router_logits, expert_idx, score, valid, offsets)
-    loss, counts, factor, work = _balance_outputs(b, router_logits.device)
+    loss, counts, buf = _balance_outputs(b, router_logits.device)
     grad = torch.empty(router_logits.shape, dtype=router_logits.dtype, device=router_logits.device)
     b.grad, b.grad_scale = grad.data_ptr(), float(grad_scale)
     _launch(N.lib.lpmm_b200_balance_forward_backward, b, router_logits.device)
