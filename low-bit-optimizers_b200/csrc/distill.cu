@@ -41,7 +41,8 @@ struct DistillArgs {
   const float* upstream;
   float* row_loss;
   RowStats* stats;
-  const float* norm;  // 1 / sum of the weights, for the mean
+  const float* norm;  // 1 / sum of the weights, for the mean; with few rows the kernels sum the weights themselves
+  int own_norm;
   long long rows, inner, outer_stride, inner_stride, grad_outer_stride, grad_inner_stride;
   int vocab, k, teacher_dtype, index_bits, upstream_per_row;
   float temperature, c;  // c = log2(e) / T
@@ -369,8 +370,21 @@ __device__ __forceinline__ void prefetch_entries(const DistillArgs& a, long long
   for (int at = lane * 128; at < a.k * size; at += 32 * 128) prefetch_l2(t + at);
 }
 
+// 1 / sum of the weights (0 if that is 0) by a warp: at most OWN_NORM_ROWS of them, a few loads per lane
+constexpr int OWN_NORM_ROWS = 256;
+__device__ __forceinline__ float own_norm(const DistillArgs& a) {
+  float w = 0.0f;
+#pragma unroll
+  for (int i = 0; i < OWN_NORM_ROWS; i += 32) {
+    const int r = i + (threadIdx.x & 31);
+    if (r < a.rows) w += a.weights[r];
+  }
+  w = Warp().sum(w);
+  return w == 0.0f ? 0.0f : 1.0f / w;
+}
+
 __device__ __forceinline__ float upstream_of(const DistillArgs& a, long long row) {
-  float up = a.scale * (a.norm ? *a.norm : 1.0f);
+  float up = a.scale * (a.norm ? *a.norm : a.own_norm ? own_norm(a) : 1.0f);
   if (a.upstream) up *= a.upstream[a.upstream_per_row ? row : 0];
   return up;
 }
@@ -466,7 +480,7 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
   RowFetch<T, MODE, KV> next;
   next.load(a, row0);
   pdl_wait();
-  const float up0 = a.scale * a.temperature * (a.norm ? *a.norm : 1.0f);
+  const float up0 = a.scale * a.temperature * (a.norm ? *a.norm : a.own_norm ? own_norm(a) : 1.0f);
   int st = 0, it = 0;
   uint32_t phase = 0;
   for (long long row = row0; row < rows; ++it, row += stride) {
@@ -1255,7 +1269,15 @@ static int distill_run(const lpmm_b200_distill* d, void* stream_) {
     if (MODE != DISTILL_GRAD && !none) LPMM_CUDA_TRY(cudaMemsetAsync(d->loss, 0, sizeof(float), stream));
     return LPMM_B200_OK;
   }
-  const bool first = MODE == DISTILL_BOTH && mean;
+  bool first = MODE == DISTILL_BOTH && mean;
+  if (first && (!d->weights || d->rows <= OWN_NORM_ROWS)) {
+    first = false;
+    a.norm = nullptr;
+    if (d->weights)
+      a.own_norm = 1;
+    else
+      a.scale = (float)((double)d->grad_scale / (double)d->rows);
+  }
   if (first) {
     distill_reduce_kernel<<<1, 1024, 0, stream>>>(nullptr, d->weights, d->rows, 1, nullptr, norm);
     LPMM_CUDA_TRY(cudaGetLastError());

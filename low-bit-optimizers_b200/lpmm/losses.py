@@ -113,9 +113,10 @@ def _distill_args(logits, teacher_logits, teacher_idx, temperature, weights, red
             raise RuntimeError(f"weights must be {tuple(lead)}, got {tuple(weights.shape)}")
         if weights.is_complex():
             raise RuntimeError(f"The type of weights is not correct: {weights.dtype}")
-        weights = weights.detach().to(torch.float32).contiguous()
-    logits, inner, outer_stride, inner_stride = _row_strides(logits.detach())
-    teacher, idx = teacher_logits.detach().contiguous(), teacher_idx.contiguous()
+        if weights.dtype != torch.float32 or not weights.is_contiguous():
+            weights = weights.to(torch.float32).contiguous()
+    logits, inner, outer_stride, inner_stride = _row_strides(logits)
+    teacher, idx = teacher_logits.contiguous(), teacher_idx.contiguous()
     d = N.Distill()
     d.logits, d.teacher, d.index = logits.data_ptr(), teacher.data_ptr(), idx.data_ptr()
     d.weights = None if weights is None else weights.data_ptr()
@@ -184,6 +185,7 @@ def topk_distillation(logits, teacher_logits, teacher_idx, temperature=1.0, weig
     return loss
 
 
+@torch.no_grad()
 def topk_distillation_with_grad(logits, teacher_logits, teacher_idx, temperature=1.0, weights=None, reduction="mean",
                                 grad_scale=1.0):
     """``topk_distillation`` and its gradient in one call: ``(loss, grad)``.
@@ -230,7 +232,7 @@ def _balance_args(router_logits, expert_idx, score, valid, offsets):
             raise RuntimeError("offsets must be one-dimensional: the sequences' starts and the last one's end")
         offsets = offsets.contiguous()
         b.offsets, b.offset_bits, b.sequences = offsets.data_ptr(), _BITS[offsets.dtype], offsets.numel() - 1
-    logits, b.inner, b.outer_stride, b.inner_stride = _row_strides(router_logits.detach())
+    logits, b.inner, b.outer_stride, b.inner_stride = _row_strides(router_logits)
     idx = expert_idx.contiguous()
     b.logits, b.index, b.tokens = logits.data_ptr(), idx.data_ptr(), logits.numel() // experts
     b.experts, b.k = experts, idx.shape[-1]
@@ -301,6 +303,7 @@ def balance_loss(router_logits, expert_idx, score="softmax", valid=None, offsets
     return loss, counts
 
 
+@torch.no_grad()
 def balance_loss_with_grad(router_logits, expert_idx, score="softmax", valid=None, offsets=None, grad_scale=1.0):
     """``balance_loss`` and its gradient in one call: ``(loss, counts, grad)``.
 
