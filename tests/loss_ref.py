@@ -34,10 +34,12 @@ def distill_row_bound(vocab, temp, w=1.0, spread=60.0):
 
 def distill_grad_bound(ref, q, p, scale, vocab, dtype, spread=60.0):
     """Elementwise: q and p are each off by the relative error of an exponential and of a sum (as above), the difference is
-    rounded once to fp32 and once to the type; below the type's smallest normal number half a step is absolute."""
+    rounded once to fp32 and once to the type; below the type's smallest normal number half a step is absolute.  An
+    exponential below 2^-126, fp32's smallest normal number, is 0: with sums of at least 1 that is less than 2^-126 of q and
+    of p, times w T (at most 1024 here): 2 * 2^-126 * 2^10 = 2^-115."""
     step = torch.finfo(dtype).eps / 2
     tiny = torch.finfo(dtype).tiny * torch.finfo(dtype).eps  # the step of the denormal range
-    return abs(scale) * (q + p) * U32 * (vocab / 128 + 64 + 16 + 8 * spread) + step * 1.001 * ref.abs() + tiny
+    return abs(scale) * ((q + p) * U32 * (vocab / 128 + 64 + 16 + 8 * spread) + 2.0 ** -115) + step * 1.001 * ref.abs() + tiny
 
 
 def balance_ref(x, idx, score="softmax", valid=None, offsets=None):

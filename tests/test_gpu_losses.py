@@ -260,19 +260,58 @@ def test_distillation_is_the_same_each_time_and_in_every_form():
     assert all(same_bits(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
 
 
-def test_distillation_rows_beyond_32_bit_offsets():
-    rows, vocab = 67200, 32000  # 2.15e9 elements
+@pytest.mark.parametrize("rows, vocab", [(67200, 32000), (2150000, 1000)])  # 2.15e9 elements
+def test_distillation_rows_beyond_32_bit_offsets(rows, vocab):
     x = torch.empty(rows, vocab, dtype=torch.bfloat16, device=device())
-    for a in range(0, rows, 8400):
-        x[a:a + 8400].normal_(generator=torch.Generator(device=device()).manual_seed(a))
+    for a in range(0, rows, rows // 8):
+        x[a:a + rows // 8].normal_(generator=torch.Generator(device=device()).manual_seed(a))
     g = torch.Generator(device=device()).manual_seed(1)
     t = torch.randn(rows, 8, device=device(), generator=g)
     idx = torch.randint(vocab, (rows, 8), device=device(), generator=g)
     loss, grad = F().topk_distillation_with_grad(x, t, idx, 1.0, reduction="none")
-    for r in (0, 33000, 67108, 67109, rows - 1):
+    edge = 2 ** 31 // vocab
+    for r in (0, rows // 2, edge - 1, edge, rows - 1):
         ref, q, p = distill_ref(x[r:r + 1], t[r:r + 1], idx[r:r + 1], 1.0)
         close(loss[r], ref[0], distill_row_bound(vocab, 1.0))
         close(grad[r:r + 1], q - p, distill_grad_bound(q - p, q, p, 1.0, vocab, torch.bfloat16))
+
+
+@pytest.mark.parametrize("temp", [2.0 ** -10, 0.01, 100.0, 1024.0])
+@pytest.mark.parametrize("rows, vocab", [(5, 700), (200, 700), (5, 20000), (160, 20000)])
+def test_distillation_far_temperatures(rows, vocab, temp):
+    """Arguments of exponentials up to 25 / T in size: that is the spread of the bounds."""
+    x, t, idx = distill_inputs(rows, vocab, 6, "fp32", seed=14)
+    loss, q, p = distill_ref(x, t, idx, temp)
+    got, grad = F().topk_distillation_with_grad(x, t, idx, temp, reduction="none")
+    spread = 60.0 + 25.0 / temp
+    close(got, loss, distill_row_bound(vocab, temp, spread=spread))
+    close(grad, temp * (q - p), distill_grad_bound(temp * (q - p), q, p, temp, vocab, torch.float32, spread=spread))
+
+
+def test_distillation_second_backward_and_changed_inputs():
+    x, t, idx = distill_inputs(7, 900, 5, "fp32", seed=15)
+    leaf = x.clone().requires_grad_()
+    loss = F().topk_distillation(leaf, t, idx, 2.0, reduction="none")
+    up = torch.linspace(-1, 2, 7, device=device())
+    (a,) = torch.autograd.grad(loss, leaf, up, retain_graph=True)
+    (b,) = torch.autograd.grad(loss, leaf, up)
+    assert same_bits(a, b)
+    _, q, p = distill_ref(x, t, idx, 2.0)
+    coef = (2.0 * up).double().cpu().view(-1, 1)
+    close(a, coef * (q - p), distill_grad_bound(coef * (q - p), coef.abs() * q, coef.abs() * p, 1.0, 900, torch.float32))
+    loss = F().topk_distillation(leaf, t, idx)
+    t.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_distillation_weights_of_other_types():
+    x, t, idx = distill_inputs(9, 300, 4, "bf16", seed=16)
+    mask = torch.arange(9, device=device()) % 3 != 0
+    want = F().topk_distillation_with_grad(x, t, idx, weights=mask.float())
+    for w in (mask, mask.int(), mask.double(), mask.bfloat16(), torch.stack([mask, mask], 1)[:, 0]):
+        got = F().topk_distillation_with_grad(x, t, idx, weights=w)
+        assert all(same_bits(a, b) for a, b in zip(want, got))
 
 
 def test_distillation_on_another_stream_and_in_graphs():
@@ -392,6 +431,40 @@ def test_balance_sequences(tokens, cuts, score):
     x, idx = balance_inputs(tokens, 40, 3, "fp32", seed=len(cuts), idx_dtype=torch.int32)
     for dt in (torch.int32, torch.int64):
         check_balance(x, idx, score, offsets=torch.tensor(cuts, dtype=dt, device=device()), grad_scale=50.0)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_balance_many_sequences(score):
+    """More sequences than offsets are kept in shared memory: some empty, some of one token, some of hundreds."""
+    g = torch.Generator().manual_seed(11)
+    sizes = torch.randint(0, 8, (3000,), generator=g)
+    sizes[::500] = 300
+    cuts = torch.cat([torch.tensor([2]), 2 + sizes.cumsum(0)])
+    x, idx = balance_inputs(int(cuts[-1]) + 5, 20, 2, "fp32", seed=12)
+    check_balance(x, idx, score, offsets=cuts.to(device()), grad_scale=10.0)
+
+
+def test_balance_tokens_beyond_32_bit_offsets():
+    tokens, experts = 8400000, 256  # 2.15e9 logits
+    g = torch.Generator(device=device()).manual_seed(1)
+    x = torch.empty(tokens, experts, dtype=torch.bfloat16, device=device())
+    for a in range(0, tokens, tokens // 8):
+        x[a:a + tokens // 8].normal_(generator=g)
+    idx = torch.randint(experts, (tokens, 1), device=device(), generator=g, dtype=torch.int32)
+    loss, counts, grad = F().balance_loss_with_grad(x, idx, grad_scale=float(tokens))
+    assert torch.equal(counts, torch.bincount(idx[:, 0], minlength=experts))
+    mass = torch.zeros(experts, dtype=torch.float64, device=device())
+    for a in range(0, tokens, tokens // 40):
+        mass += torch.softmax(x[a:a + tokens // 40].double(), 1).sum(0)
+    f = experts * counts.double() / tokens
+    ref = (f * mass).sum().cpu() / tokens
+    close(loss, ref, balance_loss_bound(ref, tokens // 2368, experts))  # tokens per warp: what is added in fp32
+    edge = 2 ** 31 // experts
+    for r in (0, edge - 1, edge, tokens - 1):
+        p = torch.softmax(x[r:r + 1].double(), 1)
+        dot = (f * p).sum(1, keepdim=True)
+        want, size = p * (f - dot), p * (f + dot)
+        close(grad[r:r + 1], want.cpu(), balance_grad_bound(want.cpu(), size.cpu(), 1.0, experts, torch.bfloat16))
 
 
 def test_balance_masks_drops_and_repeated_experts():
