@@ -48,7 +48,7 @@ struct DistillArgs {
   float temperature, c;  // c = log2(e) / T
   float scale;
   int slice;             // stream, split: columns per CTA of the cluster
-  int k_pad, hash_size;  // entries per row rounded up, slots of the table that finds an index given twice
+  int k_pad, mark_bits;  // entries per row rounded up; bits that find an index given twice
   int stages, resident;  // stream: chunks in the ring; a row stays in it for both passes.  rows: rows ahead per warp
   int slot;              // rows: bytes of a row in shared memory
   int tellers;           // stream: warps that prepare entries
@@ -241,60 +241,114 @@ struct Block {  // all threads of the CTA (at most 16 warps)
   }
 };
 
+template <typename T>
 struct Entries {
-  int* idx;    // [k_pad], -1: no entry
-  float* z;    // [k_pad] (t - tm) c: the probability is 2^z / ts
-  float* x;    // [k_pad] the student's logit
-  int* hash;   // [hash_size], -1 when not in use
-  int* twice;  // an index occurs more than once
+  int* idx;  // [k_pad], -1: no entry
+  float* z;  // [k_pad] (t - tm) c: the probability is 2^z / ts
+  T* x;      // [k_pad] the student's logit
+  static constexpr size_t BYTES = 8 + sizeof(T);
+  __device__ __forceinline__ Entries(char* p, const DistillArgs& a)
+      : idx(reinterpret_cast<int*>(p)), z(reinterpret_cast<float*>(p + 4 * a.k_pad)), x(reinterpret_cast<T*>(p + 8 * a.k_pad)) {}
 };
-
-__host__ __device__ constexpr size_t entry_bytes(int k_pad, int hash_size) { return 12 * (size_t)k_pad + 4 * (size_t)hash_size; }
-
-__device__ __forceinline__ Entries entries_at(char* p, const DistillArgs& a, int* twice) {
-  Entries e;
-  e.idx = reinterpret_cast<int*>(p);
-  e.z = reinterpret_cast<float*>(p + 4 * a.k_pad);
-  e.x = reinterpret_cast<float*>(p + 8 * a.k_pad);
-  e.hash = reinterpret_cast<int*>(p + 12 * a.k_pad);
-  e.twice = twice;
-  return e;
-}
 
 struct Teacher {
   float w, tm, ts;
   bool live;  // weight and entries: the row has a part in the loss
 };
 
-// puts i into the table; true if it was there
-__device__ __forceinline__ bool seen(int* hash, int size, int i) {
-  for (unsigned h = ((unsigned)i * 2654435761u) >> 12;; ++h) {  // ends: the table is at most half full
-    const int was = atomicCAS(&hash[h & (size - 1)], -1, i);
-    if (was == -1 || was == i) return was == i;
+// N entries k, k + step, ... of a row as they lie in memory: all loads of a kind one after another, whatever the types are,
+// and no conversion here, which would wait for its load.  What is behind the last entry has index -1.
+template <int N>
+struct RawEntries {
+  unsigned long long i_raw[N];
+  uint32_t t_raw[N];
+  __device__ __forceinline__ void load(const DistillArgs& a, long long row, int k, int step) {
+    const long long first = row * a.k;
+#pragma unroll
+    for (int j = 0; j < N; ++j) i_raw[j] = ~0ull, t_raw[j] = 0;
+    if (a.index_bits == 64) {
+      const unsigned long long* p = reinterpret_cast<const unsigned long long*>(a.index) + first;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k + j * step < a.k) i_raw[j] = p[k + j * step];
+    } else {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(a.index) + first;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k + j * step < a.k) i_raw[j] = p[k + j * step];
+    }
+    if (a.teacher_dtype == LPMM_B200_DTYPE_FP32) {
+      const uint32_t* p = reinterpret_cast<const uint32_t*>(a.teacher) + first;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k + j * step < a.k) t_raw[j] = p[k + j * step];
+    } else {
+      const unsigned short* p = reinterpret_cast<const unsigned short*>(a.teacher) + first;
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (k + j * step < a.k) t_raw[j] = p[k + j * step];
+    }
   }
-}
+  __device__ __forceinline__ long long index(const DistillArgs& a, int j) const {
+    return a.index_bits == 64 ? (long long)i_raw[j] : (long long)(int)(uint32_t)i_raw[j];
+  }
+  __device__ __forceinline__ float teacher(const DistillArgs& a, int j) const {
+    if (a.teacher_dtype == LPMM_B200_DTYPE_FP32) return __uint_as_float(t_raw[j]);
+    if (a.teacher_dtype == LPMM_B200_DTYPE_BF16) return __uint_as_float(t_raw[j] << 16);
+    return __half2float(__ushort_as_half((unsigned short)t_raw[j]));
+  }
+};
+
+// Columns of a CTA's part of a row that entries have named, a bit each (some columns share a bit where there are more than
+// `bits`, a power of two: a pair of them is then taken for one column that occurs twice, which costs a look and no more).
+// Marked and cleared entry by entry.
+struct Marks {
+  uint32_t* word;
+  int bits;
+  __device__ __forceinline__ bool mark(int column) const {
+    const unsigned c = (unsigned)column & (bits - 1);
+    return atomicOr(&word[c >> 5], 1u << (c & 31)) >> (c & 31) & 1;
+  }
+  __device__ __forceinline__ void clear(int column) const { word[((unsigned)column & (bits - 1)) >> 5] = 0; }
+};
 
 // Reads the row's entries.  GRAD: the statistics are in `st`.  The team's threads may read `e` afterwards.
 template <typename T, int MODE, typename Team>
-__device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, const T* x, Entries e, Team& team,
+__device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, const T* x, const Entries<T>& e, Team& team,
                                            const RowStats& st) {
   Teacher t;
   t.w = a.weights ? a.weights[row] : 1.0f;
   t.tm = LOWEST;
   bool any = false, bad = false;
-  if (team.rank() == 0) *e.twice = 0;
-#pragma unroll(MODE == DISTILL_LOSS ? 2 : 4)
-  for (int k = team.rank(); k < a.k; k += team.size()) {
-    const long long i = load_index(a.index, row * a.k + k, a.index_bits);
-    const float v = load_any(a.teacher, row * a.k + k, a.teacher_dtype);
-    const bool entry = i >= 0 && v != -__int_as_float(0x7f800000);
-    const bool in = entry && i < a.vocab;  // an index outside of the vocabulary is not followed
-    bad |= entry && !in;
-    any |= entry;
-    e.idx[k] = in ? (int)i : -1;
-    e.z[k] = v;
-    if (in) e.x[k] = Elem<T>::widen(x[i]);
-    if (entry) t.tm = fmaxf(t.tm, v);
+  // four entries per thread at a time, first all of their loads, then all of the logits that they point to
+  for (int k0 = team.rank(); k0 < a.k; k0 += 4 * team.size()) {
+    RawEntries<4> raw;
+    raw.load(a, row, k0, team.size());
+    float v[4];
+    uint32_t xr[4];
+    int in[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const long long i = raw.index(a, j);
+      v[j] = raw.teacher(a, j);
+      const bool entry = i >= 0 && v[j] != -__int_as_float(0x7f800000);
+      const bool inside = entry && i < a.vocab;  // an index outside of the vocabulary is not followed
+      bad |= entry && !inside;
+      any |= entry;
+      in[j] = inside ? (int)i : -1;
+      if (entry) t.tm = fmaxf(t.tm, v[j]);
+      xr[j] = 0;
+      if (inside) xr[j] = Elem<T>::raw(x + in[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = k0 + j * team.size();
+      if (k < a.k) {
+        e.idx[k] = in[j];
+        e.z[k] = v[j];
+        e.x[k] = Elem<T>::type_of(xr[j]);
+      }
+    }
   }
   t.live = team.any(any) && t.w != 0.0f;
   t.ts = 0.0f;
@@ -305,49 +359,56 @@ __device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, 
     t.tm = team.max(t.tm);
   float sum = 0.0f;
   for (int k = team.rank(); k < a.k; k += team.size()) {
-    const int i = e.idx[k];
     const float z = (e.z[k] - t.tm) * a.c;
     e.z[k] = z;
-    if (i < 0) continue;
-    sum += ex2(z);
-    if (MODE != DISTILL_LOSS && seen(e.hash, a.hash_size, i)) *e.twice = 1;
+    if (e.idx[k] >= 0) sum += ex2(z);
   }
   if (MODE == DISTILL_GRAD) {
     t.ts = st.ts;
-    team.sync();
   } else {
     t.ts = team.sum(sum);
     if (team.any(bad)) t.ts = nan_f();
   }
-  if (MODE != DISTILL_LOSS) {
-    for (int i = team.rank(); i < a.hash_size; i += team.size()) e.hash[i] = -1;
-    team.sync();
-  }
+  team.sync();
   return t;
 }
 
 // sum_k p_k (log p_k - log q_k) of a prepared row, for all threads of the team: log2 p_k = z - log2 ts
-template <typename Team>
-__device__ __forceinline__ float divergence(const DistillArgs& a, const Teacher& t, const Entries& e, Team& team,
+template <typename T, typename Team>
+__device__ __forceinline__ float divergence(const DistillArgs& a, const Teacher& t, const Entries<T>& e, Team& team,
                                             const Expo& ex, float s) {
   float sum = 0.0f;
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const float z = e.z[k], p = ex2(z);
     if (e.idx[k] < 0 || p == 0.0f) continue;
-    sum += p * (z - ex.log2_of(e.x[k]));
+    sum += p * (z - ex.log2_of(Elem<T>::widen(e.x[k])));
   }
   return LN2 * (team.sum(sum) * rcp_nr(t.ts) + (lg2(s) - lg2(t.ts)));
 }
 
-// The entries' columns within [lo, hi): q - p, written over q.  After a barrier behind the stores of q.
+// Marks the entries' columns within [lo, hi); true for a thread that found one marked.
 template <typename T, typename Team>
-__device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const Entries& e, const Team& team,
-                                              const Expo& ex, float gs, float G, float ts, int lo, int hi) {
-  const bool twice = *e.twice;
+__device__ __forceinline__ bool mark_entries(const DistillArgs& a, const Entries<T>& e, const Team& team, const Marks& marks,
+                                             int lo, int hi) {
+  bool twice = false;
+  for (int k = team.rank(); k < a.k; k += team.size()) {
+    const int i = e.idx[k];
+    if (i >= lo && i < hi) twice |= marks.mark(i - lo);
+  }
+  return twice;
+}
+
+// The entries' columns within [lo, hi): q - p, written over q.  After a barrier behind the stores of q and the marks, which
+// are cleared here.
+template <typename T, typename Team>
+__device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const Entries<T>& e, const Team& team,
+                                              const Marks& marks, bool twice, const Expo& ex, float gs, float G, float ts,
+                                              int lo, int hi) {
   const float Gp = G * rcp_nr(ts);
   for (int k = team.rank(); k < a.k; k += team.size()) {
     const int i = e.idx[k];
     if (i < lo || i >= hi) continue;
+    marks.clear(i - lo);
     float p = ex2(e.z[k]);
     if (twice) {  // an index that occurs several times: its first entry writes for all, in their order
       bool first = true;
@@ -356,7 +417,7 @@ __device__ __forceinline__ void write_entries(const DistillArgs& a, T* g, const 
       for (int j = k + 1; j < a.k; ++j)
         if (e.idx[j] == i) p += ex2(e.z[j]);
     }
-    g[i] = Elem<T>::narrow(gs * ex(e.x[k]) - Gp * p);
+    g[i] = Elem<T>::narrow(gs * ex(Elem<T>::widen(e.x[k])) - Gp * p);
   }
 }
 
@@ -403,30 +464,17 @@ __device__ __noinline__ float far_sum(const DistillArgs& a, const T* x, int lo, 
 // ---------------------------------------------------------------------------------------------
 constexpr int ROWS_MAX_WARPS = 8, ROWS_MAX_STAGES = 4, ROWS_MAX_BYTES = 16384;
 
-// What a warp loads of its next row, as it lies in memory: a conversion here would wait for the load.
+// What a warp loads of its next row
 template <typename T, int MODE, int KV>
-struct RowFetch {
-  unsigned long long i_raw[KV];
-  uint32_t t_raw[KV], edge_raw;
+struct RowFetch : RawEntries<KV> {
+  uint32_t edge_raw;
   float w, up;
   RowStats st;
   __device__ __forceinline__ void load(const DistillArgs& a, long long row) {
     const int lane = threadIdx.x & 31;
     if (row >= a.rows) return;
     w = a.weights ? a.weights[row] : 1.0f;
-    const long long first = row * a.k;
-#pragma unroll
-    for (int j = 0; j < KV; ++j) {
-      const int k = lane + 32 * j;
-      i_raw[j] = ~0ull;
-      t_raw[j] = 0;
-      if (k < a.k) {
-        i_raw[j] = a.index_bits == 64 ? reinterpret_cast<const unsigned long long*>(a.index)[first + k]
-                                      : (unsigned long long)reinterpret_cast<const uint32_t*>(a.index)[first + k];
-        t_raw[j] = a.teacher_dtype == LPMM_B200_DTYPE_FP32 ? reinterpret_cast<const uint32_t*>(a.teacher)[first + k]
-                                                           : reinterpret_cast<const unsigned short*>(a.teacher)[first + k];
-      }
-    }
+    RawEntries<KV>::load(a, row, lane, 32);
     const T* x = logits_row<T>(a, row);
     const int at = edge_of<T>(span_of(x, 0, a.vocab), lane);
     edge_raw = Elem<T>::none().x;
@@ -435,14 +483,6 @@ struct RowFetch {
       st = a.stats[row];
       up = a.upstream[a.upstream_per_row ? row : 0];
     }
-  }
-  __device__ __forceinline__ long long index(const DistillArgs& a, int j) const {
-    return a.index_bits == 64 ? (long long)i_raw[j] : (long long)(int)(uint32_t)i_raw[j];
-  }
-  __device__ __forceinline__ float teacher(const DistillArgs& a, int j) const {
-    if (a.teacher_dtype == LPMM_B200_DTYPE_FP32) return __uint_as_float(t_raw[j]);
-    if (a.teacher_dtype == LPMM_B200_DTYPE_BF16) return __uint_as_float(t_raw[j] << 16);
-    return __half2float(__ushort_as_half((unsigned short)t_raw[j]));
   }
   __device__ __forceinline__ float edge() const { return Elem<T>::of_raw(edge_raw); }
 };
@@ -675,7 +715,7 @@ struct Shape {
 
 struct StreamRow {  // what the consumers are told about a row, and what they tell
   Teacher t;
-  int skip, twice;
+  int skip;
   float m, s, G;
 };
 
@@ -687,6 +727,7 @@ struct StreamSmem {
   float2 part[2][MAX_PARTS];
   StreamRow row[2 * MAX_TELLERS];
   float2 red[2][8];
+  int twice[4];  // of row number n in twice[n & 3]
   int failed;
 };
 
@@ -738,8 +779,9 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
   char* ring = smem;
   StreamSmem& sm = *reinterpret_cast<StreamSmem*>(smem + (size_t)a.stages * CHUNK);
   char* entry_mem = smem + (size_t)a.stages * CHUNK + (sizeof(StreamSmem) + 15) / 16 * 16;
-  const size_t per_slot = entry_bytes(a.k_pad, 0);
-  int* hashes = reinterpret_cast<int*>(entry_mem + 2 * a.tellers * per_slot);
+  const size_t per_slot = Entries<T>::BYTES * a.k_pad;
+  // two sets of marks in turn where no barrier lies between the end of a row and the next one's marks
+  uint32_t* mark_words = reinterpret_cast<uint32_t*>(entry_mem + 2 * a.tellers * per_slot);
   cg::cluster_group cluster = cg::this_cluster();
   const int parts = (int)cluster.num_blocks(), part = (int)cluster.block_rank();
   const int lo = min(part * a.slice, a.vocab), hi = min(lo + a.slice, a.vocab);
@@ -756,9 +798,11 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
     }
     for (int i = 0; i < 2; ++i) mbar_init(&sm.joined[i], 1);
     sm.failed = 0;
+    for (int i = 0; i < 4; ++i) sm.twice[i] = 0;
     mbar_fence();
   }
-  for (int i = threadIdx.x; i < a.tellers * a.hash_size; i += blockDim.x) hashes[i] = -1;
+  if (MODE != DISTILL_LOSS)
+    for (int i = threadIdx.x; i < a.mark_bits / 32 * (MODE == DISTILL_GRAD ? 2 : 1); i += blockDim.x) mark_words[i] = 0;
   if (parts > 1)
     cluster.sync();
   else
@@ -813,8 +857,7 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
       if (row < a.rows) {
         const int slot = teller + (n & 1) * a.tellers;
         StreamRow& h = sm.row[slot];
-        Entries e = entries_at(entry_mem + slot * per_slot, a, &h.twice);
-        e.hash = hashes + teller * a.hash_size;
+        const Entries<T> e(entry_mem + slot * per_slot, a);
         if (n >= 2) mbar_wait(&sm.freed[slot], (n >> 1 & 1) ^ 1, &sm.failed);
         RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
         if (MODE == DISTILL_GRAD) st = a.stats[row];
@@ -838,7 +881,7 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
           float loss = 0.0f;
           if (t.live)
             loss = t.w * a.temperature * a.temperature *
-                   divergence(a, t, entries_at(entry_mem + slot * per_slot, a, nullptr), team, Expo(h.m, a.c), h.s);
+                   divergence(a, t, Entries<T>(entry_mem + slot * per_slot, a), team, Expo(h.m, a.c), h.s);
           if (lane == 0) {
             a.row_loss[before] = loss;
             a.stats[before] = RowStats{h.m, h.s, t.tm, t.ts};
@@ -853,7 +896,7 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
     const int tid = threadIdx.x;
     Consumers<CW> team(sm.red);
     int st = 0, slot = 0;
-    uint32_t phase = 0, told = 0, joins = 0;
+    uint32_t phase = 0, told = 0, joins = 0, number = 0;  // of live rows
     for (long long row = row0; row < a.rows; row += grid) {
       const T* x = logits_row<T>(a, row);
       T* g = MODE == DISTILL_LOSS ? nullptr : grad_row<T>(a, row);
@@ -932,6 +975,12 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
         if (MODE != DISTILL_LOSS) {
           const Expo ex(m, a.c);
           const float G = h.G, gs = G * rcp_nr(s);
+          const Entries<T> e(entry_mem + slot * per_slot, a);
+          const Marks marks{mark_words + (MODE == DISTILL_GRAD ? (number & 1) * (a.mark_bits / 32) : 0), a.mark_bits};
+          // the flag of row n is read behind its barrier and cleared in row n + 2: behind the barrier of row n + 1, before that
+          // of row n + 2, behind which row n + 4 sets it again
+          if (mark_entries(a, e, team, marks, lo, hi)) sm.twice[number & 3] = 1;
+          if (tid == 0) sm.twice[(number + 2) & 3] = 0;
           int s2 = MODE == DISTILL_BOTH && a.resident ? st0 : st;
           for (int i = 0; i < chunks; ++i) {
             if (MODE == DISTILL_GRAD || !a.resident) mbar_wait(&sm.full[s2], phase, &sm.failed);
@@ -959,7 +1008,8 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
           if (MODE == DISTILL_GRAD || !a.resident) st = s2;
           if (at >= 0) g[at] = E::narrow(gs * ex(edge));
           team.sync();
-          write_entries(a, g, entries_at(entry_mem + slot * per_slot, a, &h.twice), team, ex, gs, G, h.t.ts, lo, hi);
+          write_entries(a, g, e, team, marks, sm.twice[number & 3] != 0, ex, gs, G, h.t.ts, lo, hi);
+          ++number;
         }
       }
       __syncwarp();
@@ -995,10 +1045,12 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
   const int lo = min(part * a.slice, a.vocab), hi = min(lo + a.slice, a.vocab);
   const T* x = logits_row<T>(a, row);
   T* g = MODE == DISTILL_LOSS ? nullptr : grad_row<T>(a, row);
-  Entries e = entries_at(smem, a, &twice);
+  const Entries<T> e(smem, a);
+  const Marks marks{reinterpret_cast<uint32_t*>(smem + Entries<T>::BYTES * a.k_pad), a.mark_bits};
   Block team(red);
+  if (tid == 0) twice = 0;
   if (MODE != DISTILL_LOSS)
-    for (int i = tid; i < a.hash_size; i += nthr) e.hash[i] = -1;
+    for (int i = tid; i < a.mark_bits / 32; i += nthr) marks.word[i] = 0;
   __syncthreads();
   pdl_wait();
   RowStats st = {0.0f, 1.0f, 0.0f, 0.0f};
@@ -1058,6 +1110,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
   if (MODE == DISTILL_LOSS) return;
   const float G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);  // NaN for a row with invalid entries
   const float gs = G * rcp_nr(st.s);
+  if (mark_entries(a, e, team, marks, lo, hi)) twice = 1;
   {
     const Span o = span_of(g, lo, hi);
     const int at = edge_of<T>(o, tid);
@@ -1067,7 +1120,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
     for (int i = tid; i < o.vecs; i += nthr) gv[i] = ex.scaled<T>(xv[i], gs);
   }
   __syncthreads();
-  write_entries(a, g, e, team, ex, gs, G, t.ts, lo, hi);
+  write_entries(a, g, e, team, marks, twice != 0, ex, gs, G, t.ts, lo, hi);
 }
 
 // One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double.
@@ -1174,29 +1227,45 @@ static int most_clusters(int parts, int threads, size_t smem) {
   return n.load();
 }
 
+// bits for `columns` columns: up to 8 KB
+static int mark_bits(long long columns) {
+  int bits = 1024;
+  while (bits < columns && bits < 65536) bits *= 2;
+  return bits;
+}
+
 template <typename T, int MODE, int CW>
 static cudaError_t stream_launch(DistillArgs& a, long long row_bytes, bool after, cudaStream_t stream) {
   using S = Shape<MODE, CW>;
-  const size_t fixed = (sizeof(StreamSmem) + 15) / 16 * 16, told = entry_bytes(2 * a.k_pad, a.hash_size);
-  a.tellers = S::TELLERS;
-  while (a.tellers > 1 && a.tellers * told > S::ROOM / 6) --a.tellers;
-  a.stages = (int)((S::ROOM - fixed - a.tellers * told) / S::CHUNK);
-  if (a.stages > MAX_STAGES) a.stages = MAX_STAGES;
+  const size_t fixed = (sizeof(StreamSmem) + 15) / 16 * 16, told = 2 * Entries<T>::BYTES * a.k_pad;
   // With both passes in one call a row stays in the ring where it fits.  Up to 128 KB it is else copied a second time: the
   // rows under way are then less than 38 MB and still in L2 (bf16, 65536 columns: 214 us, and 235 shared by a cluster).
   // Larger rows would come from memory again; clusters of CTAs share their columns (131072: 246, and 268 copied twice).
-  const long long room = (long long)(a.stages - 1) * S::CHUNK;
+  const bool share = MODE == DISTILL_BOTH && row_bytes > 128 * 1024;
   int parts = 1;
-  if (MODE == DISTILL_BOTH && row_bytes > 128 * 1024)
-    while (parts < MAX_PARTS && row_bytes > parts * room) parts *= 2;
-  const size_t smem = a.stages * S::CHUNK + fixed + a.tellers * told;
-  const int threads = S::THREADS + 32 + 32 * a.tellers;
-  const int clusters = parts > 1 ? most_clusters<T, MODE, CW>(parts, threads, smem) : S::CTAS * num_sms();
-  if (clusters <= 0) return cudaErrorInvalidConfiguration;
-  a.slice = ((a.vocab + parts - 1) / parts + 63) / 64 * 64;
-  a.resident = MODE == DISTILL_BOTH && row_bytes <= parts * room;
-  return launch(distill_stream_kernel<T, MODE, CW>, a, (a.rows < clusters ? a.rows : clusters) * parts, threads, smem, parts,
-                after, stream);
+  for (;; parts *= 2) {
+    a.slice = ((a.vocab + parts - 1) / parts + 63) / 64 * 64;
+    a.mark_bits = MODE == DISTILL_LOSS ? 0 : mark_bits(a.slice);
+    const size_t marks = a.mark_bits / 8 * (MODE == DISTILL_GRAD ? 2 : 1);
+    a.tellers = S::TELLERS;
+    while (a.tellers > 1 && a.tellers * told > S::ROOM / 5) --a.tellers;
+    const auto stages = [&] { return (int)((S::ROOM - fixed - marks - a.tellers * told) / S::CHUNK); };
+    // long rows: as few tellers as leave the ring the most chunks
+    if (share) {
+      const int most = (int)((S::ROOM - fixed - marks - told) / S::CHUNK);
+      while (stages() < most) --a.tellers;
+    }
+    a.stages = stages() < MAX_STAGES ? stages() : MAX_STAGES;
+    a.resident = MODE == DISTILL_BOTH && row_bytes <= (long long)parts * (a.stages - 1) * S::CHUNK;
+    if (!share || a.resident || parts == MAX_PARTS) {
+      const size_t smem = a.stages * S::CHUNK + fixed + marks + a.tellers * told;
+      const int threads = S::THREADS + 32 + 32 * a.tellers;
+      const int clusters = parts > 1 ? most_clusters<T, MODE, CW>(parts, threads, smem) : S::CTAS * num_sms();
+      if (clusters <= 0) return cudaErrorInvalidConfiguration;
+      return launch(distill_stream_kernel<T, MODE, CW>, a, (a.rows < clusters ? a.rows : clusters) * parts, threads, smem,
+                    parts, after, stream);
+    }
+  }
 }
 
 // `after`: the kernel before it in the stream is this call's sum of the weights
@@ -1204,7 +1273,6 @@ template <typename T, int MODE>
 static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t stream) {
   constexpr int VE = Elem<T>::VE;
   const long long row_bytes = (long long)a.vocab * sizeof(T);
-  const size_t entries = entry_bytes(a.k_pad, a.hash_size);
   const int sms = num_sms();
   // A warp per row up to 16 KB for the loss (bf16, 8192 columns: 171 us against 179 of the streaming kernel; fp32, 4096: 128
   // against 165), up to 8 KB with the gradient (4096 columns: 309 against 375; 8192: 420 against 309).
@@ -1224,10 +1292,10 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   }
   if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES / 2) {
     // Four consuming warps per CTA or eight, measured with 64 entries and 512 MB of logits (us, four / eight): the loss of
-    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; gradient 12000 194 / 200,
-    // 131072 196 / 190; both 8192 309 / -, 12000 296 / 355, 20000 270 / 292, 32000 236 / 237, 50257 255 / 233, fp32 12000
+    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; the gradient
+    // alone is about the same (12000 194 / 200, 131072 196 / 190) and has eight; both 8192 309 / -, 12000 296 / 355, 20000 270 / 292, 32000 236 / 237, 50257 255 / 233, fp32 12000
     // 221 / 204.  Many entries take the room of the smaller ring.
-    const bool few = a.k <= 256 && row_bytes <= (MODE == DISTILL_BOTH ? 40 * 1024 : 128 * 1024);
+    const bool few = a.k <= 256 && row_bytes <= (MODE == DISTILL_BOTH ? 40 : MODE == DISTILL_LOSS ? 128 : 0) * 1024;
     const cudaError_t e = few ? stream_launch<T, MODE, 4>(a, row_bytes, after, stream)
                               : stream_launch<T, MODE, 8>(a, row_bytes, after, stream);
     if (e != cudaErrorInvalidConfiguration) return e;
@@ -1239,7 +1307,9 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   a.slice = ((vecs + parts - 1) / parts + 7) / 8 * 8 * VE;
   const int per = a.slice / VE;
   const int threads = per >= 2048 ? 512 : per >= 512 ? 256 : 128;
-  return launch(distill_split_kernel<T, MODE>, a, a.rows * parts, threads, entries, parts, after, stream);
+  a.mark_bits = MODE == DISTILL_LOSS ? 0 : mark_bits(a.slice);
+  return launch(distill_split_kernel<T, MODE>, a, a.rows * parts, threads, Entries<T>::BYTES * a.k_pad + a.mark_bits / 8, parts,
+                after, stream);
 }
 
 template <int MODE>
@@ -1263,8 +1333,6 @@ static int distill_run(const lpmm_b200_distill* d, void* stream_) {
   a.scale = d->grad_scale;
   a.grad_outer_stride = d->grad_outer_stride, a.grad_inner_stride = d->grad_inner_stride;
   a.k_pad = (a.k + 3) / 4 * 4;
-  if (MODE != DISTILL_LOSS)
-    for (a.hash_size = 32; a.hash_size < 2 * a.k;) a.hash_size *= 2;
   if (d->rows == 0) {
     if (MODE != DISTILL_GRAD && !none) LPMM_CUDA_TRY(cudaMemsetAsync(d->loss, 0, sizeof(float), stream));
     return LPMM_B200_OK;

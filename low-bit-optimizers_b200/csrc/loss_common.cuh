@@ -17,6 +17,7 @@ struct Elem<float> {
   static __device__ __forceinline__ float narrow(float v) { return v; }
   static __device__ __forceinline__ uint32_t raw(const float* p) { return *reinterpret_cast<const uint32_t*>(p); }
   static __device__ __forceinline__ float of_raw(uint32_t w) { return __uint_as_float(w); }
+  static __device__ __forceinline__ float type_of(uint32_t w) { return __uint_as_float(w); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
   template <int N>
   static __device__ __forceinline__ float maximum(const uint4* u) {  // NaN is passed over, here and below
@@ -42,6 +43,7 @@ struct Elem<__nv_bfloat16> {
   static __device__ __forceinline__ __nv_bfloat16 narrow(float v) { return __float2bfloat16_rn(v); }
   static __device__ __forceinline__ uint32_t raw(const __nv_bfloat16* p) { return *reinterpret_cast<const unsigned short*>(p); }
   static __device__ __forceinline__ float of_raw(uint32_t w) { return __uint_as_float(w << 16); }
+  static __device__ __forceinline__ __nv_bfloat16 type_of(uint32_t w) { return __ushort_as_bfloat16((unsigned short)w); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
   template <int N>
   static __device__ __forceinline__ float maximum(const uint4* u) {
@@ -73,6 +75,7 @@ struct Elem<__half> {
   static __device__ __forceinline__ __half narrow(float v) { return __float2half_rn(v); }
   static __device__ __forceinline__ uint32_t raw(const __half* p) { return *reinterpret_cast<const unsigned short*>(p); }
   static __device__ __forceinline__ float of_raw(uint32_t w) { return __half2float(__ushort_as_half((unsigned short)w)); }
+  static __device__ __forceinline__ __half type_of(uint32_t w) { return __ushort_as_half((unsigned short)w); }
   static __device__ __forceinline__ uint4 none() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
   template <int N>
   static __device__ __forceinline__ float maximum(const uint4* u) {

@@ -40,13 +40,13 @@ def _row_strides(t):
     if t.is_contiguous():
         return t, 1, n, 0
     if t.dim() == 1:
-        return t.contiguous(), 1, n, 0
+        return t.detach().contiguous(), 1, n, 0
     if t.stride(-1) == 1 or n == 1:
         if t.dim() == 2:
             return t, 1, t.stride(0), 0
         if t.dim() == 3:
             return (t, t.shape[1], t.stride(0), t.stride(1)) if t.shape[1] > 1 else (t, 1, t.stride(0), 0)
-    return t.contiguous(), 1, n, 0
+    return t.detach().contiguous(), 1, n, 0
 
 
 def _grad_of(logits, d):
@@ -185,7 +185,6 @@ def topk_distillation(logits, teacher_logits, teacher_idx, temperature=1.0, weig
     return loss
 
 
-@torch.no_grad()
 def topk_distillation_with_grad(logits, teacher_logits, teacher_idx, temperature=1.0, weights=None, reduction="mean",
                                 grad_scale=1.0):
     """``topk_distillation`` and its gradient in one call: ``(loss, grad)``.
@@ -303,7 +302,6 @@ def balance_loss(router_logits, expert_idx, score="softmax", valid=None, offsets
     return loss, counts
 
 
-@torch.no_grad()
 def balance_loss_with_grad(router_logits, expert_idx, score="softmax", valid=None, offsets=None, grad_scale=1.0):
     """``balance_loss`` and its gradient in one call: ``(loss, counts, grad)``.
 
