@@ -129,6 +129,7 @@ __device__ __forceinline__ void count_phase(const BalanceArgs& a, const Offsets&
   __syncthreads();
   int lo, hi;
   tile.run(lo, hi);
+  const unsigned kth = 0xffffffffu / (unsigned)a.k + 1;  // x / k = the upper half of x * kth, for x < 2^15 and 1 < k <= 2^10
   for (int r = lo; r < hi;) {
     const Stretch t = stretch_at(a, o, r, hi);
     if (t.s >= 0) {
@@ -146,7 +147,8 @@ __device__ __forceinline__ void count_phase(const BalanceArgs& a, const Offsets&
           for (int u = 0; u < 4; ++u) e[u] = i + 32 * u < entries ? load_index(a.index, first + i + 32 * u, a.index_bits) : -1;
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
-            if (e[u] < 0 || (a.valid && !(ok >> ((unsigned)(i + 32 * u) / (unsigned)a.k) & 1))) continue;
+            if (e[u] < 0) continue;
+            if (a.valid && !(ok >> (a.k == 1 ? (unsigned)(i + 32 * u) : __umulhi(i + 32 * u, kth)) & 1)) continue;
             if (e[u] >= a.experts)
               atomicOr(&a.bad[t.s], 1);
             else if (set >= 0)
