@@ -2,7 +2,7 @@
 (rank-1, group, wider codes, larger groups), the factored second moment, momentum SGD per tensor and
 fused, next to the fused AdamW step on the same shapes.  Seeded synthetic inputs.
 
-    python benchmarks/paths.py [--iters 10] [--only SUBSTRING] [--big]
+    python benchmarks/paths.py [--iters 10] [--only SUBSTRING] [--big | --copy | --pack | --losses]
 
 One line per case: parameters, CUDA-event time per step (after 3 warm-up steps), wall time per step,
 parameters per second.  ``LPMM_SGD_PER_TENSOR=1`` in the environment times the per-tensor SGD launches
@@ -179,6 +179,59 @@ def pack_rate(n=1 << 28, iters=10):
         print(f"{label} of {n} values (incl. the output allocation): {ms:.3f} ms, {4.5 * n / ms / 1e6:.0f} GB/s", flush=True)
 
 
+def losses(iters=20, only=None):
+    """The training losses of ``lpmm.functional`` on the vocabularies of the two parameter lists and on routers: bytes that a
+    call cannot do without (logits read once, their gradient written once) over CUDA-event time."""
+    F, dev = lpmm.functional, torch.device("cuda:0")
+    gen = torch.Generator(device=dev).manual_seed(0)
+
+    def distill(rows, vocab, k, dtype):
+        x = torch.randn(rows, vocab, device=dev, generator=gen).mul_(2.5).to(dtype)
+        t = torch.randn(rows, k, device=dev, generator=gen).bfloat16()
+        i = torch.rand(rows, vocab, device=dev, generator=gen).topk(k).indices.int()
+        return x, t, i
+
+    def route(tokens, experts, k, dtype):
+        x = torch.randn(tokens, experts, device=dev, generator=gen).to(dtype)
+        return x, x.float().topk(k).indices
+
+    def backward(fn, x):
+        return torch.autograd.grad(fn(x.requires_grad_()), x)
+
+    cases = []
+    for rows, vocab, k, dtype in ((16384, 32000, 64, torch.bfloat16), (4096, 50257, 32, torch.float32),
+                                  (2048, 131072, 256, torch.bfloat16), (7, 50257, 50, torch.bfloat16)):
+        for how, fn in (("loss", lambda x, t, i: F.topk_distillation(x.detach(), t, i, 2.0)),
+                        ("loss and gradient", lambda x, t, i: F.topk_distillation_with_grad(x, t, i, 2.0)),
+                        ("loss.backward()", lambda x, t, i: backward(lambda x: F.topk_distillation(x, t, i, 2.0), x))):
+            cases.append((f"distillation {rows} x {vocab} {str(dtype)[6:]}, {k} entries: {how}", distill,
+                          (rows, vocab, k, dtype), fn, 1 if how == "loss" else 2))
+    for tokens, experts, k, dtype in ((16384, 64, 2, torch.float32), (131072, 256, 8, torch.bfloat16), (48, 8, 2, torch.float16)):
+        for how, fn in (("loss", lambda x, i: F.balance_loss(x.detach(), i)),
+                        ("loss and gradient", lambda x, i: F.balance_loss_with_grad(x, i)),
+                        ("loss.backward()", lambda x, i: backward(lambda x: F.balance_loss(x, i)[0], x))):
+            cases.append((f"balance {tokens} x {experts} {str(dtype)[6:]}, {k} chosen: {how}", route,
+                          (tokens, experts, k, dtype), fn, 1 if how == "loss" else 2))
+    for name, make, sizes, fn, passes in cases:
+        if only is not None and only not in name:
+            continue
+        args = make(*sizes)
+        for _ in range(3):
+            fn(*args)
+        torch.cuda.synchronize()
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(iters):
+            fn(*args)
+        b.record()
+        torch.cuda.synchronize()
+        ms = a.elapsed_time(b) / iters
+        nbytes = passes * args[0].numel() * args[0].element_size() + sum(t.numel() * t.element_size() for t in args[1:])
+        print(f"{name}: {ms * 1e3:.1f} us, {nbytes / ms / 1e6:.0f} GB/s", flush=True)
+        del args
+        torch.cuda.empty_cache()
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--iters", type=int, default=10)
@@ -186,6 +239,7 @@ def main():
     ap.add_argument("--big", action="store_true", help="the LLaMA-7B-shaped list instead (needs ~70 GB)")
     ap.add_argument("--copy", action="store_true", help="time torch's device copy instead (burst and sustained)")
     ap.add_argument("--pack", action="store_true", help="time the standalone 4-bit pack / unpack of 2^28 values instead")
+    ap.add_argument("--losses", action="store_true", help="time the training losses of lpmm.functional instead")
     a = ap.parse_args()
     if not torch.cuda.is_available():
         raise SystemExit("needs a CUDA device")
@@ -193,6 +247,8 @@ def main():
         return copy_rate()
     if a.pack:
         return pack_rate()
+    if a.losses:
+        return losses(only=a.only)
     for name, kind, shapes, kw in (big_cases() if a.big else cases()):
         if a.only is None or a.only in name:
             run(name, kind, shapes, kw, a.iters)
