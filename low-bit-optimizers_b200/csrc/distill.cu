@@ -1292,9 +1292,9 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   }
   if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES / 2) {
     // Four consuming warps per CTA or eight, measured with 64 entries and 512 MB of logits (us, four / eight): the loss of
-    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; the gradient
-    // alone is about the same (12000 194 / 200, 131072 196 / 190) and has eight; both 8192 309 / -, 12000 296 / 355, 20000 270 / 292, 32000 236 / 237, 50257 255 / 233, fp32 12000
-    // 221 / 204.  Many entries take the room of the smaller ring.
+    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; both 12000 296 / 355, 20000
+    // 270 / 292, 32000 236 / 237, 50257 255 / 233, fp32 12000 221 / 204; the gradient alone is about the same (12000 194 / 200,
+    // 131072 196 / 190) and has eight.  Many entries take the room of the smaller ring.
     const bool few = a.k <= 256 && row_bytes <= (MODE == DISTILL_BOTH ? 40 : MODE == DISTILL_LOSS ? 128 : 0) * 1024;
     const cudaError_t e = few ? stream_launch<T, MODE, 4>(a, row_bytes, after, stream)
                               : stream_launch<T, MODE, 8>(a, row_bytes, after, stream);
