@@ -53,8 +53,13 @@ def _grad_of(logits, d):
     """A tensor for the gradient of ``logits`` (the tensor that ``d`` describes), its strides in ``d``.  Contiguous where
     that puts every row to the 16-byte boundaries as the logits' row lies to them, which the kernels' wide accesses
     need; else with up to 16 bytes between rows."""
-    n, size = logits.shape[-1], logits.element_size()
-    off, wide = logits.data_ptr() % 16 // size, 16 // size
+    n, at = logits.shape[-1], d.logits or 0
+    if at % 16 == 0 and logits.is_contiguous():
+        grad = torch.empty_like(logits)
+        d.grad, d.grad_outer_stride, d.grad_inner_stride = grad.data_ptr(), d.outer_stride, d.inner_stride
+        return grad
+    size = logits.element_size()
+    off, wide = at % 16 // size, 16 // size
     if d.inner == 1:
         inner, outer = 0, n + (d.outer_stride - n) % wide
         odd = outer != n
@@ -71,17 +76,21 @@ def _grad_of(logits, d):
         else:
             grad = grad[off:].view(logits.shape)
     else:
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
     d.grad, d.grad_outer_stride, d.grad_inner_stride = grad.data_ptr(), outer, inner
     return grad
 
 
+# the handle of a device's current stream; building a Stream object for it takes ten times as long
+_stream_of = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
 def _launch(fn, args, device):
     if device.index == torch.cuda.current_device():
-        N.check(fn(args, torch.cuda.current_stream().cuda_stream))
+        N.check(fn(args, _stream_of(device.index)))
     else:
         with torch.cuda.device(device):
-            N.check(fn(args, torch.cuda.current_stream().cuda_stream))
+            N.check(fn(args, _stream_of(device.index)))
 
 
 # ----------------------------------------------------------------------------------------------
@@ -270,7 +279,7 @@ class _BalanceLoss(torch.autograd.Function):
     def backward(ctx, upstream, _):
         router_logits, expert_idx, valid, offsets, counts = ctx.saved_tensors
         b, kept = _balance_args(router_logits, expert_idx, ctx.score, valid, offsets)
-        grad = torch.empty(router_logits.shape, dtype=router_logits.dtype, device=router_logits.device)
+        grad = torch.empty_like(router_logits, memory_format=torch.contiguous_format)
         upstream = upstream.to(torch.float32).contiguous()
         b.grad, b.upstream, b.counts, b.factor = grad.data_ptr(), upstream.data_ptr(), counts.data_ptr(), ctx.factor
         _launch(N.lib.lpmm_b200_balance_backward, b, router_logits.device)
@@ -309,7 +318,7 @@ def balance_loss_with_grad(router_logits, expert_idx, score="softmax", valid=Non
     ``router_logits``: a new contiguous tensor of their shape and type.  Nothing takes part in autograd."""
     b, kept = _balance_args(router_logits, expert_idx, score, valid, offsets)
     loss, counts, buf = _balance_outputs(b, router_logits.device)
-    grad = torch.empty(router_logits.shape, dtype=router_logits.dtype, device=router_logits.device)
+    grad = torch.empty_like(router_logits, memory_format=torch.contiguous_format)
     b.grad, b.grad_scale = grad.data_ptr(), float(grad_scale)
     _launch(N.lib.lpmm_b200_balance_forward_backward, b, router_logits.device)
     return loss, counts, grad

@@ -145,7 +145,7 @@ def test_gradient_layout(make, dtype):
     """The gradient's rows are where the structure says, apart, inside their storage, and like the logits' rows to 16 bytes."""
     t = make(torch.zeros(4, 5, 203, dtype=dtype))
     got, inner, outer, step = L._row_strides(t)
-    d = N.Distill(inner=inner, outer_stride=outer, inner_stride=step, rows=got.numel() // got.shape[-1])
+    d = N.Distill(logits=got.data_ptr(), inner=inner, outer_stride=outer, inner_stride=step, rows=got.numel() // got.shape[-1])
     g = L._grad_of(got, d)
     assert g.shape == t.shape and g.dtype == dtype
     flat = g.as_strided((g.untyped_storage().nbytes() // g.element_size(),), (1,), 0).fill_(-1)
