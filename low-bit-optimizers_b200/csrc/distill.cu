@@ -709,7 +709,7 @@ template <int MODE, int CW>
 struct Shape {
   static constexpr int CHUNK = 2048 * CW, THREADS = 32 * CW;
   static constexpr int CTAS = CW == 8 ? 2 : MODE == DISTILL_BOTH ? 4 : 5;
-  static constexpr int TELLERS = CW == 8 ? 4 : MODE == DISTILL_BOTH ? 2 : 1;
+  static constexpr int TELLERS = CW == 8 ? 4 : 1;
   static constexpr size_t ROOM = 227 * 1024 / CTAS - 1024;
 };
 
@@ -1292,10 +1292,11 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   }
   if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES / 2) {
     // Four consuming warps per CTA or eight, measured with 64 entries and 512 MB of logits (us, four / eight): the loss of
-    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; both 12000 296 / 355, 20000
-    // 270 / 292, 32000 236 / 237, 50257 255 / 233, fp32 12000 221 / 204; the gradient alone is about the same (12000 194 / 200,
-    // 131072 196 / 190) and has eight.  Many entries take the room of the smaller ring.
-    const bool few = a.k <= 256 && row_bytes <= (MODE == DISTILL_BOTH ? 40 : MODE == DISTILL_LOSS ? 128 : 0) * 1024;
+    // bf16 rows of 12000 columns 138 / 210, 32000 107 / 126, 65536 102 / 105, 131072 102 / 96; both, bf16 12000 274 / 353,
+    // 20000 246 / 289, 32000 226 / 232, 50257 258 / 234, fp32 12000 197 / 212, 16000 222 / 198 (fp32 has half the
+    // exponentials per byte to hide); the gradient alone is about the same (12000 194 / 200, 131072 196 / 190) and has eight.
+    const long long most = MODE == DISTILL_LOSS ? 128 : MODE == DISTILL_GRAD ? 0 : sizeof(T) == 2 ? 64 : 48;
+    const bool few = a.k <= 256 && row_bytes <= most * 1024;  // more entries take the room of the smaller ring
     const cudaError_t e = few ? stream_launch<T, MODE, 4>(a, row_bytes, after, stream)
                               : stream_launch<T, MODE, 8>(a, row_bytes, after, stream);
     if (e != cudaErrorInvalidConfiguration) return e;
