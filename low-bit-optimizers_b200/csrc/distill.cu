@@ -59,7 +59,7 @@ constexpr float FAR = 1e38f;
 constexpr float LN2 = 0.6931471805599453f;
 
 // Where |m c| is beyond FAR (rows of the type's lowest value, above all) fp32 cannot hold M: such a row is done with
-// (x - m) c instead, which is exact there.
+// (x - m) c instead, which stays in range.
 __device__ __forceinline__ float ref_of(float m, float c) { return fmaxf(m * c, -FAR); }
 __device__ __forceinline__ bool far_off(float m, float c) { return !(fabsf(m * c) <= FAR); }
 
@@ -460,7 +460,9 @@ __device__ __noinline__ float far_sum(const DistillArgs& a, const T* x, int lo, 
 
 // ---------------------------------------------------------------------------------------------
 // rows: every warp takes rows of its own; their logits are copied into its slots of shared memory some rows ahead, the
-// entries of the next row are loaded into registers (KV per lane)
+// entries of the next row are loaded into registers (KV per lane).  A warp needs no barrier with others, and a gathered logit
+// comes from shared memory.  Bound by instructions: about 900 per row and warp beside its columns (loss and gradient of
+// 512 MB of bf16 logits, 64 entries: 4096 columns 311 us = 0.53 of the copy rate, 1000 columns 421 us = 0.42).
 // ---------------------------------------------------------------------------------------------
 constexpr int ROWS_MAX_WARPS = 8, ROWS_MAX_STAGES = 4, ROWS_MAX_BYTES = 16384;
 
@@ -697,7 +699,11 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
 
 // ---------------------------------------------------------------------------------------------
 // stream: persistent CTAs, or clusters of them that share the columns of a row; one warp copies the rows into a ring of
-// chunks, a few prepare the entries of the next rows, eight take the passes
+// chunks, one to four prepare the entries of rows to come, four or eight take the passes.  Gathered logits, the teacher's
+// softmax and the losses, a chain of latencies per row, are thus off the path that the row's columns take.
+// Bound by memory and, for 16-bit types, by how many chunks' latencies four warps per scheduler hide (the pipe of the
+// exponentials is 54-65 % busy).  512 MB of logits, 64 entries: loss, bf16, 32000 columns 106 us = 0.78 of the copy rate
+// (fp32 96 us, 0.85); gradient 207 us, 0.79; both 226 us, 0.73 (fp32 207 us, 0.79).
 // ---------------------------------------------------------------------------------------------
 constexpr int PER = 4;  // vectors per consuming thread and chunk
 constexpr int MAX_STAGES = 14, MAX_TELLERS = 4, MAX_PARTS = 8;
@@ -1029,7 +1035,9 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
 }
 
 // ---------------------------------------------------------------------------------------------
-// split: one CTA, or one cluster of CTAs that share the columns, per row
+// split: one CTA, or one cluster of CTAs that share the columns, per row: fewer rows than SMs, or more entries than the
+// kernel for short rows takes.  Bound by latencies: entries, the gathered logits, the row, two barriers of the cluster (7 rows
+// of 50257 bf16 columns, both: 13 us).
 // ---------------------------------------------------------------------------------------------
 template <typename T, int MODE>
 __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a) {
@@ -1123,7 +1131,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
   write_entries(a, g, e, team, marks, twice != 0, ex, gs, G, t.ts, lo, hi);
 }
 
-// One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double.
+// One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double (3 us).
 __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __restrict__ row_loss,
                                                               const float* __restrict__ weights, long long rows, int mean,
                                                               float* __restrict__ loss, float* __restrict__ norm) {
@@ -1274,9 +1282,11 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   constexpr int VE = Elem<T>::VE;
   const long long row_bytes = (long long)a.vocab * sizeof(T);
   const int sms = num_sms();
-  // A warp per row up to 16 KB for the loss (bf16, 8192 columns: 171 us against 179 of the streaming kernel; fp32, 4096: 128
-  // against 165), up to 8 KB with the gradient (4096 columns: 309 against 375; 8192: 420 against 309).
-  if (row_bytes <= (MODE == DISTILL_LOSS ? ROWS_MAX_BYTES : ROWS_MAX_BYTES / 2) && a.k <= 256) {
+  // A warp per row up to 16 KB for the loss, 12 KB for the gradient, 8 KB for both (us, here / streaming: loss, bf16 8192 columns
+  // 171 / 179, fp32 4096 130 / 155; gradient, bf16 6000 221 / 262, 8192 250 / 238; both, bf16 4096 311 / 420, 6000 362 / 373,
+  // fp32 4096 341 / 234).
+  constexpr long long ROW = MODE == DISTILL_LOSS ? ROWS_MAX_BYTES : MODE == DISTILL_GRAD ? ROWS_MAX_BYTES / 4 * 3 : ROWS_MAX_BYTES / 2;
+  if (row_bytes <= ROW && a.k <= 256) {
     a.slot = (int)((row_bytes + 15) / 16 * 16);
     int warps = ROWS_MAX_WARPS, ctas = a.k <= 64 ? 3 : 2;
     a.stages = ROWS_MAX_STAGES;

@@ -107,6 +107,26 @@ def test_distillation_temperature_weights_reduction(dtype, temp, reduction):
     check_distill(x, t, idx, temp, None, reduction)
 
 
+@pytest.mark.parametrize("idx_dtype", [torch.int32, torch.int64])
+@pytest.mark.parametrize("tdtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows, vocab, k", [(9, 500, 33), (9, 500, 130), (9, 500, 260), (7, 9000, 70), (150, 9000, 70)])
+def test_distillation_types_of_the_entries(rows, vocab, k, tdtype, idx_dtype):
+    x, t, idx = distill_inputs(rows, vocab, k, "bf16", seed=17, idx_dtype=idx_dtype, tdtype=tdtype)
+    idx[:, 1::5] = -1
+    t[:, 2::7] = -INF
+    check_distill(x, t, idx, 1.5, None, "sum")
+
+
+@pytest.mark.parametrize("rows", [255, 256, 257, 600])
+@pytest.mark.parametrize("vocab", [700, 10000])
+def test_distillation_mean_over_weights(rows, vocab):
+    x, t, idx = distill_inputs(rows, vocab, 5, "fp32", seed=18)
+    w = torch.rand(rows, generator=torch.Generator().manual_seed(2)).to(device())
+    w[::7] = 0
+    check_distill(x, t, idx, 2.0, w, "mean")
+    check_distill(x, t, idx, 2.0, None, "mean")
+
+
 # (copies of the twelve rows, columns): each kernel, the vocabulary within one CTA's columns and shared by a cluster
 REGIMES = [(1, 1001), (150, 1001), (1, 4095), (1, 20011), (13, 9003), (26, 30001), (13, 70003)]
 
