@@ -444,10 +444,12 @@ __device__ __forceinline__ float own_norm(const DistillArgs& a) {
   return w == 0.0f ? 0.0f : 1.0f / w;
 }
 
+// The gradient's factor that all rows share.  For whole warps: own_norm adds up over the lanes.
+__device__ __forceinline__ float shared_factor(const DistillArgs& a) {
+  return a.scale * a.temperature * (a.norm ? *a.norm : a.own_norm ? own_norm(a) : 1.0f);
+}
 __device__ __forceinline__ float upstream_of(const DistillArgs& a, long long row) {
-  float up = a.scale * (a.norm ? *a.norm : a.own_norm ? own_norm(a) : 1.0f);
-  if (a.upstream) up *= a.upstream[a.upstream_per_row ? row : 0];
-  return up;
+  return a.upstream ? a.upstream[a.upstream_per_row ? row : 0] : 1.0f;
 }
 
 // Statistics of a row whose maximum lies beyond FAR, from its logits in memory.
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
   RowFetch<T, MODE, KV> next;
   next.load(a, row0);
   pdl_wait();
-  const float up0 = a.scale * a.temperature * (a.norm ? *a.norm : a.own_norm ? own_norm(a) : 1.0f);
+  const float up0 = MODE == DISTILL_LOSS ? 0.0f : shared_factor(a);
   int st = 0, it = 0;
   uint32_t phase = 0;
   for (long long row = row0; row < rows; ++it, row += stride) {
@@ -854,6 +856,7 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
     __syncwarp();
   } else if (warp > CW) {  // the entries
     pdl_wait();  // *norm
+    const float up0 = MODE == DISTILL_LOSS ? 0.0f : shared_factor(a);
     Warp team;
     const int teller = warp - CW - 1;
     const long long step = a.tellers * grid;
@@ -872,7 +875,7 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
           h.t = t;
           h.skip = t.w == 0.0f;
           if (MODE == DISTILL_GRAD) h.m = st.m, h.s = st.s;
-          if (MODE != DISTILL_LOSS) h.G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);
+          if (MODE != DISTILL_LOSS) h.G = up0 * upstream_of(a, row) * t.w + (t.ts - t.ts);
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.told[slot]);
@@ -1116,7 +1119,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
     }
   }
   if (MODE == DISTILL_LOSS) return;
-  const float G = upstream_of(a, row) * t.w * a.temperature + (t.ts - t.ts);  // NaN for a row with invalid entries
+  const float G = shared_factor(a) * upstream_of(a, row) * t.w + (t.ts - t.ts);  // NaN for a row with invalid entries
   const float gs = G * rcp_nr(st.s);
   if (mark_entries(a, e, team, marks, lo, hi)) twice = 1;
   {
