@@ -91,6 +91,12 @@ __device__ __forceinline__ double factor_of(const BalanceArgs& a, int s) {
   return n == 0.0 ? 0.0 : (double)a.experts / ((double)a.k * n * n);
 }
 
+// An expert's count for the gradient, less that of the first expert: c_e - sum_j c_j p_j does not change with a constant, for the
+// scores add up to 1, and in a well balanced sequence the differences are small next to the counts: even counts give exactly 0.
+__device__ __forceinline__ float count_of(const BalanceArgs& a, int s, int e) {
+  return (float)(long long)(__ldcg(&a.counts[cell(a, s, e)]) - __ldcg(&a.counts[cell(a, s, 0)]));
+}
+
 // A CTA's part of the tokens.  What its first and its last sequence gather is put together in shared memory (they may
 // have many tokens here); sequences between them lie within the CTA and go straight to memory.
 struct Tile {
@@ -231,8 +237,8 @@ __device__ __forceinline__ void score_phase(const BalanceArgs& a, const Offsets&
   if (GRAD) {
     if (SUM) pdl_wait();  // the counts
     for (int e = threadIdx.x; e < a.experts; e += blockDim.x) {
-      if (tile.first >= 0) counts[e] = (float)__ldcg(&a.counts[cell(a, tile.first, e)]);
-      if (tile.last >= 0) counts[a.experts + e] = (float)__ldcg(&a.counts[cell(a, tile.last, e)]);
+      if (tile.first >= 0) counts[e] = count_of(a, tile.first, e);
+      if (tile.last >= 0) counts[a.experts + e] = count_of(a, tile.last, e);
     }
   }
   __syncthreads();
@@ -258,7 +264,7 @@ __device__ __forceinline__ void score_phase(const BalanceArgs& a, const Offsets&
       for (int h = 0; h < 2; ++h) {
         const int i = 2 * n + h, col = (i / V * G + gl) * V + i % V;
         if (GRAD && any && i < JV && col < a.experts)
-          v[h] = set >= 0 ? counts[set * a.experts + col] : (float)__ldcg(&a.counts[cell(a, t.s, col)]);
+          v[h] = set >= 0 ? counts[set * a.experts + col] : count_of(a, t.s, col);
       }
       c[n] = f2_pack(v[0], v[1]);
       acc[n] = zero;

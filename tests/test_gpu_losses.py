@@ -579,6 +579,29 @@ def test_balance_gradient_against_differences():
         assert abs((up - down) / (2 * h) - (grad.double() * d).sum().item()) < tol
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens, experts", [(64, 8), (8192, 16), (20000, 125)])
+def test_balance_of_an_even_router(tokens, experts, score):
+    """Even counts: no gradient at all.  One assignment moved: the gradient is that of counts (1, -1, 0, ...), to a few roundings
+    of its own size and not of the counts'."""
+    x = torch.randn(tokens, experts, generator=torch.Generator().manual_seed(13)).to(device())
+    idx = (torch.arange(tokens, device=device()) % experts)[:, None]
+    if tokens % experts == 0:
+        _, counts, grad = F().balance_loss_with_grad(x, idx, score, grad_scale=float(tokens))
+        assert counts.unique().numel() == 1 and not grad.any()
+    idx[0] = 1
+    check_balance(x, idx, score, grad_scale=float(tokens))
+    _, counts, grad = F().balance_loss_with_grad(x, idx, score, grad_scale=float(tokens))
+    x64 = x.double().cpu()
+    logp = torch.log_softmax(x64 if score == "softmax" else torch.nn.functional.logsigmoid(x64), 1)
+    p, c = logp.exp(), (counts - counts[0]).double().cpu()
+    slope = 1.0 if score == "softmax" else torch.sigmoid(-x64)
+    dot = (c * p).sum(1, keepdim=True)
+    ref = experts / tokens * p * (c - dot) * slope
+    close(grad, ref, balance_grad_bound(ref, experts / tokens * p * (c.abs() + (c.abs() * p).sum(1, keepdim=True)) * slope, 1.0,
+                                        experts, torch.float32))
+
+
 def test_balance_counts_do_not_take_part_in_autograd():
     x, idx = balance_inputs(20, 8, 2, "fp32")
     loss, counts = F().balance_loss(x.requires_grad_(), idx)
