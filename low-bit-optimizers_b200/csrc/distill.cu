@@ -373,6 +373,12 @@ __device__ __forceinline__ Teacher prepare(const DistillArgs& a, long long row, 
   return t;
 }
 
+// sum = sum_k 2^z_k (z_k - log2 e_k).  One logarithm, of the quotient: two that nearly cancel would each be rounded at their size.
+__device__ __forceinline__ float divergence_of(float sum, float s, float ts) {
+  const float r = rcp_nr(ts);
+  return LN2 * (sum * r) + logf(s * r);
+}
+
 // sum_k p_k (log p_k - log q_k) of a prepared row, for all threads of the team: log2 p_k = z - log2 ts
 template <typename T, typename Team>
 __device__ __forceinline__ float divergence(const DistillArgs& a, const Teacher& t, const Entries<T>& e, Team& team,
@@ -383,7 +389,7 @@ __device__ __forceinline__ float divergence(const DistillArgs& a, const Teacher&
     if (e.idx[k] < 0 || p == 0.0f) continue;
     sum += p * (z - ex.log2_of(Elem<T>::widen(e.x[k])));
   }
-  return LN2 * (team.sum(sum) * rcp_nr(t.ts) + (lg2(s) - lg2(t.ts)));
+  return divergence_of(team.sum(sum), s, t.ts);
 }
 
 // Marks the entries' columns within [lo, hi); true for a thread that found one marked.
@@ -608,7 +614,7 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
           if (r.s == 0.0f) r.s = nan_f();  // every logit -inf: no distribution
         }
         if (lane == 0) {
-          a.row_loss[row] = f.w * a.temperature * a.temperature * LN2 * (sum * rcp_nr(ts) + (lg2(r.s) - lg2(ts)));
+          a.row_loss[row] = f.w * a.temperature * a.temperature * divergence_of(sum, r.s, ts);
           a.stats[row] = RowStats{r.m, r.s, tm, ts};
         }
       }

@@ -110,13 +110,6 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// log2 by the hardware instruction (absolute error 2^-22 near 1, relative elsewhere)
-__device__ __forceinline__ float lg2(float x) {
-  float r;
-  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 __device__ __forceinline__ float load_any(const void* p, long long i, int dtype) {
   if (dtype == LPMM_B200_DTYPE_FP32) return reinterpret_cast<const float*>(p)[i];
   if (dtype == LPMM_B200_DTYPE_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
