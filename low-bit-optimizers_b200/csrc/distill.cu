@@ -55,11 +55,13 @@ struct DistillArgs {
 };
 
 constexpr float LOWEST = -3.402823466e38f;
-constexpr float FAR = 1e38f;
+constexpr float FAR = 16777216.0f;  // 2^24
 constexpr float LN2 = 0.6931471805599453f;
 
-// Where |m c| is beyond FAR (rows of the type's lowest value, above all) fp32 cannot hold M: such a row is done with
-// (x - m) c instead, which stays in range.
+// The exponent at x = m is what the rounding of M left of m c: at most 1 up to |m c| = FAR, beyond it soon more than an
+// exponential can hold.  A running maximum below -FAR (columns at a mask's value, whatever that is) therefore counts as -FAR:
+// its terms are 2^(x c + FAR), next to nothing.  A row whose own maximum lies beyond FAR to either side is done with
+// (x - m) c instead.
 __device__ __forceinline__ float ref_of(float m, float c) { return fmaxf(m * c, -FAR); }
 __device__ __forceinline__ bool far_off(float m, float c) { return !(fabsf(m * c) <= FAR); }
 

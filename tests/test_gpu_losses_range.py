@@ -1,0 +1,68 @@
+"""The training losses on a B200 where values, lengths or calls leave the ordinary: against the 64-bit restatements of
+``loss_ref.py`` with their bounds, and against themselves."""
+import pytest
+import torch
+
+from gpu_helpers import device
+from test_gpu_losses import DT, INF, REGIMES, check_distill_copies, distill_inputs
+
+pytestmark = pytest.mark.gpu
+
+
+# ----------------------------------------------------------------------------------------------
+# columns at a mask's finite value
+# ----------------------------------------------------------------------------------------------
+def masked_inputs(vocab, k, dtype, fill):
+    """Twelve rows with columns at `fill`; the entries lie where the student has ordinary logits."""
+    x, t, idx = distill_inputs(12, vocab, k, dtype, seed=21)
+    g = torch.Generator().manual_seed(22)
+    low = torch.finfo(DT[dtype]).min if fill == "lowest" else fill
+    live = torch.ones(12, vocab, dtype=torch.bool)
+    live[0, :vocab * 3 // 5] = False            # a thread's first columns
+    live[1, :-9] = False                        # all but the last ones
+    live[2, 9:] = False                         # all but the first ones
+    live[3, ::2] = False                        # every other one
+    live[4, vocab // 4:vocab // 2 + 64] = False  # whole parts of a cluster
+    live[6] = torch.rand(vocab, generator=g) < 0.1
+    live[6, 0] = True
+    live[8, :-1] = False                        # all but one
+    live[9] = live[1]
+    live[11, vocab // 2:] = False
+    for r in range(12):
+        at = torch.arange(vocab)[live[r]]
+        idx[r] = at[torch.randint(len(at), (k,), generator=g)]  # some of them several times
+    x[~live.to(device())] = low
+    x[5] = low                                  # nothing but masked columns: uniform
+    x[9, :vocab // 2] = low / 2                 # two mask values
+    x[10, idx[10, 0]] = abs(low)                # the largest one far above the others: certain
+    t[10, 1:] = -INF
+    w = torch.ones(12, device=device())
+    w[3], w[11] = 0.5, -2.0
+    return x, t, idx, w
+
+
+@pytest.mark.parametrize("fill", [-1e9, -1e10, -1e12, -1e20, -1e30, "lowest"])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("copies, vocab", REGIMES)
+def test_distillation_finite_masks(copies, vocab, dtype, fill):
+    x, t, idx, w = masked_inputs(vocab, 8, dtype, fill)
+    for temp in (0.25, 0.5, 1.0, 2.0, 5.0, 8.0, 20.0, 100.0):
+        check_distill_copies(copies, x, t, idx, temp, w, "none")
+
+
+@pytest.mark.parametrize("fill", [-1e10, -1e30])
+@pytest.mark.parametrize("copies, vocab", REGIMES)
+def test_distillation_finite_masks_many_entries(copies, vocab, fill):
+    x, t, idx, w = masked_inputs(vocab, 300, "bf16", fill)
+    for temp in (1.0, 5.0):
+        check_distill_copies(copies, x, t, idx, temp, w, "sum")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("copies, vocab", REGIMES)
+def test_distillation_rows_of_minus_infinity_at_high_temperatures(copies, vocab, dtype):
+    """No distribution, whatever the temperature: NaN, and the other rows as they are."""
+    x, t, idx = distill_inputs(12, vocab, 4, dtype, seed=23)
+    x[7] = -INF
+    for temp in (1.0, 8.0, 1024.0):
+        check_distill_copies(copies, x, t, idx, temp, torch.ones(12, device=device()), "none")
