@@ -534,7 +534,7 @@ typedef struct lpmm_b200_balance {
   const void* offsets;     /* [sequences + 1], offset_bits wide, or NULL (sequences = 1)                                */
   const float* upstream;   /* backward only: [sequences]                                                                */
   float* loss;             /* [sequences] (not for backward)                                                            */
-  int64_t* counts;         /* [sequences, experts]: written by forward, read by backward                                */
+  int64_t* counts;         /* [sequences, experts]: written by forward, read by backward, in between left as they are   */
   float* factor;           /* [sequences]: experts / (k n^2), written by forward, read by backward                      */
   void* work;              /* lpmm_b200_balance_work_bytes, 8-byte aligned (not for backward); directly behind counts   */
                            /* saves a clearing operation                                                                */
@@ -543,6 +543,7 @@ typedef struct lpmm_b200_balance {
   int32_t dtype, index_bits, offset_bits, score;
   float grad_scale;
   int32_t reserved;
+  int64_t* counts_out;     /* NULL, or [sequences, experts]: the counts once more, to hand on (not for backward)        */
 } lpmm_b200_balance;
 
 int64_t lpmm_b200_balance_work_bytes(int64_t experts, int64_t sequences);

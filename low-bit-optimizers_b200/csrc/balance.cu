@@ -30,6 +30,7 @@ struct BalanceArgs {
   const float* upstream;
   float* loss;
   unsigned long long* counts;  // [sequences, experts]
+  unsigned long long* counts_out;  // the same for the caller to hand on, or nullptr
   float* factor;
   unsigned long long* psum;    // [sequences, experts] summed scores in units of 2^-shift
   unsigned long long* sizes;   // valid tokens per sequence
@@ -411,7 +412,7 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// Loss and factor of the sequences.  Reads what other CTAs have written; the loads of a thread are independent of one
+// Loss and factor of the sequences, and the second copy of their counts.  Reads what other CTAs have written; the loads of a thread are independent of one
 // another.  A sequence has a warp, or, where there is one sequence only, the CTA (`red`: double[32]).
 __device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int step, double* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -420,8 +421,11 @@ __device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int 
     double sum = 0.0;
     const int from = one ? threadIdx.x : lane, by = one ? blockDim.x : 32;
 #pragma unroll 4
-    for (int e = from; e < a.experts; e += by)
-      sum += (double)__ldcg(&a.counts[cell(a, s, e)]) * (double)__ldcg(&a.psum[cell(a, s, e)]);
+    for (int e = from; e < a.experts; e += by) {
+      const unsigned long long c = __ldcg(&a.counts[cell(a, s, e)]);
+      sum += (double)c * (double)__ldcg(&a.psum[cell(a, s, e)]);
+      if (a.counts_out) a.counts_out[cell(a, s, e)] = c;
+    }
     const double f = factor_of(a, s);
     const int nan = __ldcg(&a.bad[s]) & 2;
     sum = warp_sum(sum);
@@ -622,6 +626,7 @@ static int balance_run(const lpmm_b200_balance* b, void* stream_) {
   a.logits = b->logits, a.grad = b->grad, a.index = b->index, a.valid = b->valid, a.offsets = b->offsets;
   a.upstream = b->upstream, a.loss = b->loss, a.factor = b->factor;
   a.counts = reinterpret_cast<unsigned long long*>(b->counts);
+  a.counts_out = reinterpret_cast<unsigned long long*>(b->counts_out);
   const BalanceLayout l = balance_layout(b->experts, b->sequences);
   if (SUM) {
     char* work = reinterpret_cast<char*>(b->work);

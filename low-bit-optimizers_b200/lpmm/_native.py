@@ -74,7 +74,7 @@ class Balance(ctypes.Structure):
                 + [(n, ctypes.c_int64) for n in ("tokens", "inner", "outer_stride", "inner_stride", "experts", "k",
                                                  "sequences")]
                 + [(n, ctypes.c_int32) for n in ("dtype", "index_bits", "offset_bits", "score")]
-                + [("grad_scale", ctypes.c_float), ("reserved", ctypes.c_int32)])
+                + [("grad_scale", ctypes.c_float), ("reserved", ctypes.c_int32), ("counts_out", ctypes.c_void_p)])
 
 
 STATE_FP32, STATE_GROUP4, STATE_RANK1_4, STATE_FACTORED = 0, 1, 2, 3

@@ -249,7 +249,8 @@ def _balance_args(router_logits, expert_idx, score, valid, offsets):
 
 
 def _balance_outputs(b, device):
-    """Loss, counts, and the buffer that holds the counts, the workspace behind them and the gradient's factors."""
+    """Loss, counts, and the buffer that holds what belongs to the call: counts that the backward pass reads (the caller may do
+    with the returned ones as it likes), the workspace behind them and the gradient's factors."""
     s, e = b.sequences, b.experts
     cells = s * e
     nbytes = N.lib.lpmm_b200_balance_work_bytes(e, s)  # a multiple of 16
@@ -259,8 +260,9 @@ def _balance_outputs(b, device):
     loss = torch.empty((s,) if b.offsets else (), dtype=torch.float32, device=device)
     at = buf.data_ptr()
     b.counts, b.work, b.factor, b.loss = at, at + 8 * cells, at + 8 * cells + nbytes, loss.data_ptr()
-    counts = buf[:cells]
-    return loss, counts.view(s, e) if b.offsets else counts, buf
+    counts = torch.empty((s, e) if b.offsets else (e,), dtype=torch.int64, device=device)
+    b.counts_out = counts.data_ptr()
+    return loss, counts, buf
 
 
 class _BalanceLoss(torch.autograd.Function):
@@ -270,18 +272,18 @@ class _BalanceLoss(torch.autograd.Function):
         loss, counts, ctx.buf = _balance_outputs(b, router_logits.device)
         _launch(N.lib.lpmm_b200_balance_forward, b, router_logits.device)
         ctx.mark_non_differentiable(counts)
-        ctx.save_for_backward(router_logits, expert_idx, valid, offsets, counts)
-        ctx.factor, ctx.score = b.factor, score
+        ctx.save_for_backward(router_logits, expert_idx, valid, offsets)
+        ctx.counts, ctx.factor, ctx.score = b.counts, b.factor, score
         return loss, counts
 
     @staticmethod
     @once_differentiable
     def backward(ctx, upstream, _):
-        router_logits, expert_idx, valid, offsets, counts = ctx.saved_tensors
+        router_logits, expert_idx, valid, offsets = ctx.saved_tensors
         b, kept = _balance_args(router_logits, expert_idx, ctx.score, valid, offsets)
         grad = torch.empty_like(router_logits, memory_format=torch.contiguous_format)
         upstream = upstream.to(torch.float32).contiguous()
-        b.grad, b.upstream, b.counts, b.factor = grad.data_ptr(), upstream.data_ptr(), counts.data_ptr(), ctx.factor
+        b.grad, b.upstream, b.counts, b.factor = grad.data_ptr(), upstream.data_ptr(), ctx.counts, ctx.factor
         _launch(N.lib.lpmm_b200_balance_backward, b, router_logits.device)
         return grad, None, None, None, None
 

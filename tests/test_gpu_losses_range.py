@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from gpu_helpers import device
-from test_gpu_losses import DT, INF, REGIMES, check_distill_copies, distill_inputs
+from test_gpu_losses import DT, F, INF, REGIMES, balance_inputs, check_distill_copies, distill_inputs, same_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,29 @@ def test_distillation_rows_of_minus_infinity_at_high_temperatures(copies, vocab,
     x[7] = -INF
     for temp in (1.0, 8.0, 1024.0):
         check_distill_copies(copies, x, t, idx, temp, torch.ones(12, device=device()), "none")
+
+
+# ----------------------------------------------------------------------------------------------
+# what the caller does with the counts
+# ----------------------------------------------------------------------------------------------
+# one CTA, a cluster, several launches whose last CTA adds up, more sequences than that
+@pytest.mark.parametrize("tokens, experts, sequences", [(48, 8, 0), (48, 8, 3), (3000, 64, 0), (3000, 64, 5), (30000, 64, 0),
+                                                        (30000, 64, 7), (30000, 64, 100)])
+def test_balance_gradient_does_not_read_the_returned_counts(tokens, experts, sequences):
+    x, idx = balance_inputs(tokens, experts, 2, "fp32", seed=24)
+    offsets = torch.linspace(0, tokens, sequences + 1, device=device()).long() if sequences else None
+    ends = [0, tokens] if offsets is None else offsets.tolist()
+    want_counts = torch.stack([torch.bincount(idx[a:b].reshape(-1), minlength=experts) for a, b in zip(ends[:-1], ends[1:])])
+    assert torch.equal(F().balance_loss_with_grad(x, idx, offsets=offsets)[1].view(-1, experts), want_counts)
+    x.requires_grad_()
+    grads, losses = [], []
+    for change in (lambda c: None, lambda c: c.data.mul_(2),  # as a collective over ranks leaves them, past autograd's record
+                   lambda c: c.zero_()):
+        loss, counts = F().balance_loss(x, idx, offsets=offsets)
+        assert torch.equal(counts.view(-1, experts), want_counts)
+        losses.append(loss.detach())
+        change(counts)
+        grads.append(torch.autograd.grad(loss.sum(), x)[0])
+    assert grads[0].any()
+    for same in (grads, losses):
+        assert same_bits(same[0], same[1]) and same_bits(same[0], same[2])

@@ -1,0 +1,39 @@
+"""Host side of the training losses, without a GPU: which buffers the forms share, which calls are refused."""
+import pytest
+import torch
+
+from lpmm import functional as F
+from lpmm import losses as L
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The public functions on CPU tensors: the CUDA check is left out and launches are recorded."""
+    calls = []
+    monkeypatch.setattr(L, "_check_cuda", lambda t, name: None)
+    monkeypatch.setattr(L, "_launch", lambda fn, args, device: calls.append((fn.__name__, args)))
+    return calls
+
+
+@pytest.mark.parametrize("offsets", [None, torch.tensor([0, 2, 6])])
+def test_returned_counts_are_not_what_backward_reads(host, offsets):
+    x, idx = torch.randn(6, 8, requires_grad=True), torch.zeros(6, 2, dtype=torch.int64)
+    loss, counts = F.balance_loss(x, idx, offsets=offsets)
+    name, forward = host.pop()
+    assert name == "lpmm_b200_balance_forward" and forward.counts_out == counts.data_ptr()
+    cells = 8 * (1 if offsets is None else 2)
+    assert counts.numel() == cells and counts.untyped_storage().nbytes() == 8 * cells
+    assert not counts.data_ptr() <= forward.counts < counts.data_ptr() + 8 * cells
+    counts.zero_()
+    loss.sum().backward()
+    name, backward = host.pop()
+    assert name == "lpmm_b200_balance_backward"
+    assert (backward.counts, backward.factor, backward.counts_out) == (forward.counts, forward.factor, None)
+
+
+def test_returned_counts_keep_no_workspace(host):
+    x, idx = torch.randn(6, 8), torch.zeros(6, 2, dtype=torch.int64)
+    for call in (F.balance_loss, F.balance_loss_with_grad):
+        counts = call(x, idx)[1]
+        assert counts.untyped_storage().nbytes() == 64
+        assert host.pop()[1].counts_out == counts.data_ptr()
