@@ -475,6 +475,7 @@ __device__ __noinline__ float far_sum(const DistillArgs& a, const T* x, int lo, 
 // 512 MB of bf16 logits, 64 entries: 4096 columns 311 us = 0.53 of the copy rate, 1000 columns 421 us = 0.42).
 // ---------------------------------------------------------------------------------------------
 constexpr int ROWS_MAX_WARPS = 8, ROWS_MAX_STAGES = 4, ROWS_MAX_BYTES = 16384;
+constexpr size_t rows_room(int ctas) { return 227 * 1024 / ctas - 2048; }  // shared memory of a CTA
 
 // What a warp loads of its next row
 template <typename T, int MODE, int KV>
@@ -1194,11 +1195,14 @@ static int distill_check(const lpmm_b200_distill* d, int mode) {
   return LPMM_B200_OK;
 }
 
+// `most`: the most shared memory that any call gives this kernel.  The limit belongs to the kernel on the device, and other
+// threads launch it too: set to one call's size it would refuse another's.
 template <typename K>
-static cudaError_t launch(K kernel, const DistillArgs& a, long long grid, int threads, size_t smem, int cluster, bool after,
-                          cudaStream_t stream) {
+static cudaError_t launch(K kernel, const DistillArgs& a, long long grid, int threads, size_t smem, size_t most, int cluster,
+                          bool after, cudaStream_t stream) {
+  if (smem > most) return cudaErrorInvalidValue;
   if (smem > 40 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
     if (e != cudaSuccess) return e;
   }
   cudaLaunchConfig_t cfg = {};
@@ -1231,7 +1235,8 @@ static int most_clusters(int parts, int threads, size_t smem) {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   std::atomic<int>& n = known[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3][threads / 32 - CW - 1];
   if (n.load() == 0) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, CW>::ROOM) != cudaSuccess)
+      return 0;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(Shape<MODE, CW>::CTAS * num_sms() / parts * parts), cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
@@ -1282,7 +1287,7 @@ static cudaError_t stream_launch(DistillArgs& a, long long row_bytes, bool after
       const int clusters = parts > 1 ? most_clusters<T, MODE, CW>(parts, threads, smem) : S::CTAS * num_sms();
       if (clusters <= 0) return cudaErrorInvalidConfiguration;
       return launch(distill_stream_kernel<T, MODE, CW>, a, (a.rows < clusters ? a.rows : clusters) * parts, threads, smem,
-                    parts, after, stream);
+                    S::ROOM, parts, after, stream);
     }
   }
 }
@@ -1302,14 +1307,14 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
     int warps = ROWS_MAX_WARPS, ctas = a.k <= 64 ? 3 : 2;
     a.stages = ROWS_MAX_STAGES;
     const auto bytes = [&] { return (size_t)warps * a.stages * a.slot; };
-    const auto room = [&] { return (size_t)(227 * 1024 / ctas - 2048); };
+    const auto room = [&] { return rows_room(ctas); };
     while (a.stages > 2 && bytes() > room()) --a.stages;
     if (bytes() > room()) ctas = 2;
     while (bytes() > room()) --warps;
     long long grid = (a.rows + warps - 1) / warps;
     if (grid > ctas * sms) grid = ctas * sms;
-    if (a.k <= 64) return launch(distill_rows_kernel<T, MODE, 2>, a, grid, warps * 32, bytes(), 1, after, stream);
-    return launch(distill_rows_kernel<T, MODE, 8>, a, grid, warps * 32, bytes(), 1, after, stream);
+    if (a.k <= 64) return launch(distill_rows_kernel<T, MODE, 2>, a, grid, warps * 32, bytes(), rows_room(2), 1, after, stream);
+    return launch(distill_rows_kernel<T, MODE, 8>, a, grid, warps * 32, bytes(), rows_room(2), 1, after, stream);
   }
   if (a.rows >= sms && row_bytes > ROWS_MAX_BYTES / 2) {
     // Four consuming warps per CTA or eight, measured with 64 entries and 512 MB of logits (us, four / eight): the loss of
@@ -1330,8 +1335,8 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
   const int per = a.slice / VE;
   const int threads = per >= 2048 ? 512 : per >= 512 ? 256 : 128;
   a.mark_bits = MODE == DISTILL_LOSS ? 0 : mark_bits(a.slice);
-  return launch(distill_split_kernel<T, MODE>, a, a.rows * parts, threads, Entries<T>::BYTES * a.k_pad + a.mark_bits / 8, parts,
-                after, stream);
+  return launch(distill_split_kernel<T, MODE>, a, a.rows * parts, threads, Entries<T>::BYTES * a.k_pad + a.mark_bits / 8,
+                Entries<T>::BYTES * MAX_K + 65536 / 8, parts, after, stream);
 }
 
 template <int MODE>

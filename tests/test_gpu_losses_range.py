@@ -1,5 +1,7 @@
 """The training losses on a B200 where values, lengths or calls leave the ordinary: against the 64-bit restatements of
 ``loss_ref.py`` with their bounds, and against themselves."""
+import threading
+
 import pytest
 import torch
 
@@ -92,3 +94,36 @@ def test_balance_gradient_does_not_read_the_returned_counts(tokens, experts, seq
     assert grads[0].any()
     for same in (grads, losses):
         assert same_bits(same[0], same[1]) and same_bits(same[0], same[2])
+
+
+# ----------------------------------------------------------------------------------------------
+# two host threads at a time
+# ----------------------------------------------------------------------------------------------
+# calls that take one kernel with different amounts of shared memory: short rows, a ring of small chunks, one of large chunks,
+# clusters
+@pytest.mark.parametrize("sizes", [((300, 1000, 8), (300, 4000, 8)), ((200, 12000, 8), (200, 20000, 250)),
+                                   ((160, 40000, 8), (160, 60000, 1000)), ((160, 131072, 8), (160, 100000, 1000))])
+def test_distillation_from_two_threads(sizes):
+    inputs = [distill_inputs(*s, "bf16", seed=25 + i) for i, s in enumerate(sizes)]
+    want = [F().topk_distillation_with_grad(*v, reduction="none") for v in inputs]
+    torch.cuda.synchronize()
+    errors = []
+
+    def work(v, ref):
+        try:
+            torch.cuda.set_device(device())
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(2000):
+                    got = F().topk_distillation_with_grad(*v, reduction="none")
+            stream.synchronize()
+            assert all(same_bits(a, b) for a, b in zip(ref, got))
+        except Exception as e:  # noqa: BLE001 - handed to the test's own thread
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(v, w)) for v, w in zip(inputs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
