@@ -1226,29 +1226,30 @@ static cudaError_t launch(K kernel, const DistillArgs& a, long long grid, int th
   return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
-// how many clusters of `parts` CTAs the GPU holds at a time (asked once per kernel, size and device)
+// How many clusters of `parts` CTAs the GPU holds at a time with all the shared memory that a call may give them, which does for
+// every call: asked once per kernel, cluster, number of tellers and device.  0: none, or no answer; then it is asked again.
 template <typename T, int MODE, int CW>
-static int most_clusters(int parts, int threads, size_t smem) {
+static int most_clusters(int parts, int threads) {
   const auto kernel = distill_stream_kernel<T, MODE, CW>;
   static std::atomic<int> known[64][4][MAX_TELLERS + 1];  // 0: not asked yet
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   std::atomic<int>& n = known[dev][parts == 2 ? 1 : parts == 4 ? 2 : 3][threads / 32 - CW - 1];
-  if (n.load() == 0) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, CW>::ROOM) != cudaSuccess)
-      return 0;
+  int got = n.load();
+  if (got == 0) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(Shape<MODE, CW>::CTAS * num_sms() / parts * parts), cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = Shape<MODE, CW>::ROOM;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = parts, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr, cfg.numAttrs = 1;
-    int got = 0;
-    if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) got = 0;
-    n.store(got > 0 ? got : -1);
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Shape<MODE, CW>::ROOM) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess || got < 0)
+      got = 0;
+    if (got > 0) n.store(got);
   }
-  return n.load();
+  return got;
 }
 
 // bits for `columns` columns: up to 8 KB
@@ -1284,7 +1285,7 @@ static cudaError_t stream_launch(DistillArgs& a, long long row_bytes, bool after
     if (!share || a.resident || parts == MAX_PARTS) {
       const size_t smem = a.stages * S::CHUNK + fixed + marks + a.tellers * told;
       const int threads = S::THREADS + 32 + 32 * a.tellers;
-      const int clusters = parts > 1 ? most_clusters<T, MODE, CW>(parts, threads, smem) : S::CTAS * num_sms();
+      const int clusters = parts > 1 ? most_clusters<T, MODE, CW>(parts, threads) : S::CTAS * num_sms();
       if (clusters <= 0) return cudaErrorInvalidConfiguration;
       return launch(distill_stream_kernel<T, MODE, CW>, a, (a.rows < clusters ? a.rows : clusters) * parts, threads, smem,
                     S::ROOM, parts, after, stream);
@@ -1326,6 +1327,7 @@ static cudaError_t distill_launch(DistillArgs& a, bool after, cudaStream_t strea
     const cudaError_t e = few ? stream_launch<T, MODE, 4>(a, row_bytes, after, stream)
                               : stream_launch<T, MODE, 8>(a, row_bytes, after, stream);
     if (e != cudaErrorInvalidConfiguration) return e;
+    cudaGetLastError();  // the kernel below takes the call; the next one to ask for the last error shall not find this
   }
   // few rows: their columns are shared by clusters of up to 8 CTAs, so that all SMs have work
   int parts = 1;
