@@ -524,8 +524,8 @@ int lpmm_b200_distill_forward_backward(const lpmm_b200_distill* d, void* stream)
  * offsets[s+1]); tokens of no sequence and tokens that are not valid are not looked at and have gradient 0; a sequence
  * without valid tokens has loss 0.  A negative expert index is a dropped assignment: not counted.  An index >=
  * experts makes its sequence's loss and gradient NaN, offsets that descend or leave the range make every loss NaN;
- * nothing out of range is accessed.  Counts are whole-number atomics; sums of scores are fp32 within a run of tokens of
- * one warp and 64-bit whole numbers beyond: results do not depend on how the work is scheduled. */
+ * nothing out of range is accessed.  Counts are whole-number atomics; sums of scores are fp32 within a run of at most
+ * 512 tokens and 64-bit whole numbers beyond: results do not depend on how the work is scheduled. */
 typedef struct lpmm_b200_balance {
   const void* logits;      /* row r begins at element (r / inner) * outer_stride + (r % inner) * inner_stride           */
   void* grad;              /* [tokens, experts] contiguous, type of the logits (not for forward)                        */

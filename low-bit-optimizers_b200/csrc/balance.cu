@@ -6,8 +6,8 @@
 //
 // The gradient needs the counts, not the summed scores, so loss and gradient share one pass over the logits once the
 // indices are counted.  A token's logits lie in the registers of up to 32 lanes, some tokens per warp at a time; a warp
-// walks a contiguous run of tokens and sums the scores of its columns in registers, in fp32.  Those sums (a run has at
-// most some hundred tokens) meet as 64-bit whole numbers, in units of 2^-shift with tokens * 2^shift < 2^62: atomics on
+// walks a contiguous run of tokens and sums the scores of its columns in registers, in fp32.  Those sums (of MAX_RUN tokens at
+// most, so that their rounding does not grow with the batch) meet as 64-bit whole numbers, in units of 2^-shift with tokens * 2^shift < 2^62: atomics on
 // them give the same result in any order, and what is rounded off is far below fp32 of the sum.
 // Bound by memory for large batches (a logit is read once, a gradient written once), by launches for small ones: these
 // are done in one launch of a CTA or a cluster, larger ones in three (clear, count, scores; the last CTA adds up).
@@ -20,6 +20,7 @@ namespace cg = cooperative_groups;
 namespace lpmm_b200 {
 
 constexpr int MAX_WARPS = 16;
+constexpr int MAX_RUN = 512;  // tokens whose scores are summed in fp32: reached from 1.2 million tokens on
 
 struct BalanceArgs {
   const void* logits;
@@ -250,7 +251,8 @@ __device__ __forceinline__ void score_phase(const BalanceArgs& a, const Offsets&
   const f2 log2e = f2_splat(LOG2E), zero = f2_splat(0.0f);
 
   for (int r0 = lo; r0 < hi;) {
-    const Stretch t = stretch_at(a, o, r0, hi);
+    Stretch t = stretch_at(a, o, r0, hi);
+    if (SUM) t.end = min(t.end, r0 + MAX_RUN);
     const bool any = t.s >= 0;
     Raw<T, V, J, U> next;
     next.load(a, r0, t.end, any, per, gi, gl);

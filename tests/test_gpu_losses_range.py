@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from gpu_helpers import device
-from test_gpu_losses import DT, F, INF, REGIMES, balance_inputs, check_distill_copies, distill_inputs, same_bits
+from loss_ref import U32, balance_loss_bound
+from test_gpu_losses import DT, F, INF, REGIMES, balance_inputs, check_distill_copies, close, distill_inputs, same_bits
 
 pytestmark = pytest.mark.gpu
 
@@ -94,6 +95,42 @@ def test_balance_gradient_does_not_read_the_returned_counts(tokens, experts, seq
     assert grads[0].any()
     for same in (grads, losses):
         assert same_bits(same[0], same[1]) and same_bits(same[0], same[2])
+
+
+# ----------------------------------------------------------------------------------------------
+# many tokens: what is added in fp32 has a bound of its own
+# ----------------------------------------------------------------------------------------------
+def many_tokens(row, tokens, k=1):
+    """`tokens` times the same row of logits (one in memory), and experts drawn at random."""
+    g = torch.Generator(device=device()).manual_seed(26)
+    idx = torch.randint(row.numel(), (tokens, k), device=device(), generator=g, dtype=torch.int32)
+    return row.to(device())[None].expand(tokens, -1), idx
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens", [1 << 23, 1 << 26])
+def test_balance_loss_of_many_even_tokens(tokens, score):
+    """All scores 1 / 248, loss exactly 1.  Exponentials of 0, sums of 1 and (for sigmoid, all 0.5) of 0.5 are exact; a reciprocal
+    is off by 2 roundings, a product by one, at most 512 additions of a run by one each, 5 across the lanes, the whole numbers by less
+    than one, the result by one; for sigmoid 3 more for 0.5."""
+    x, idx = many_tokens(torch.zeros(248, dtype=torch.bfloat16), tokens)
+    loss, counts = F().balance_loss(x, idx, score)
+    close(loss, torch.ones((), dtype=torch.float64), (512 + 2 + 1 + 5 + 1 + 1 + 3) * U32)
+    assert torch.equal(counts, torch.bincount(idx[:, 0], minlength=248))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("tokens, cuts", [(1 << 26, None), (9000001, [5, 4000000, 4000003, 9000000])])
+def test_balance_loss_of_many_tokens(tokens, cuts, score):
+    row = torch.randn(248, generator=torch.Generator().manual_seed(27)).bfloat16()
+    x, idx = many_tokens(row, tokens, 2)
+    offsets = None if cuts is None else torch.tensor(cuts, device=device())
+    loss, counts = F().balance_loss(x, idx, score, offsets=offsets)
+    x64 = row.double()
+    p = torch.softmax(x64 if score == "softmax" else torch.nn.functional.logsigmoid(x64), 0)
+    c = counts.double().cpu().view(-1, 248)
+    ref = (248 * c / c.sum(1, keepdim=True) * p).sum(1).view(loss.shape)
+    close(loss, ref, balance_loss_bound(ref, 0, 248))  # its constant part has the 512 additions of a run
 
 
 # ----------------------------------------------------------------------------------------------
