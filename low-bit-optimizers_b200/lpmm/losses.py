@@ -7,6 +7,7 @@ the logits are then read once instead of twice, and nothing of autograd runs.  B
 of the logits' device and synchronise nothing.
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
@@ -30,6 +31,15 @@ def _check_tensor(t, name, dtypes, like):
         raise RuntimeError(f"{name} is on {t.device}, the logits are on {like.device}")
     if t.dtype not in dtypes:
         raise RuntimeError(f"The type of {name} is not correct: {t.dtype}")
+
+
+def _refuse_tangents(tensors):
+    """The differentiable forms have no forward-mode derivative: a dual tensor would lose its tangent in silence."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open, so there are no dual tensors
+        return
+    for t, name in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError(f"{name} carries a forward-mode tangent, which is not supported: only the backward pass is")
 
 
 def _row_strides(t):
@@ -181,7 +191,9 @@ def topk_distillation(logits, teacher_logits, teacher_idx, temperature=1.0, weig
     ``reduction``: ``"none"`` gives ``[...]`` losses, ``"sum"`` their sum, ``"mean"`` the sum over the sum of the
     weights (0 if that is 0).  The loss is fp32, the gradient has the logits' type and is rounded once.
 
-    An index of V or more makes its row's loss and gradient NaN.  Results do not depend on scheduling."""
+    An index of V or more makes its row's loss and gradient NaN.  Results do not depend on scheduling.  Tensors with
+    forward-mode tangents are refused."""
+    _refuse_tangents(((logits, "logits"), (teacher_logits, "teacher_logits"), (weights, "weights")))
     if torch.is_grad_enabled():
         for t, name in ((teacher_logits, "teacher_logits"), (weights, "weights")):
             if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -304,7 +316,8 @@ def balance_loss(router_logits, expert_idx, score="softmax", valid=None, offsets
     tokens has loss 0.  Loss fp32, counts int64, gradient of the logits' type, rounded once.
 
     An index of E or more makes its sequence's loss and gradient NaN, offsets that descend or leave the range make every
-    loss NaN.  Results do not depend on scheduling."""
+    loss NaN.  Results do not depend on scheduling.  Logits with a forward-mode tangent are refused."""
+    _refuse_tangents(((router_logits, "router_logits"),))
     if torch.is_grad_enabled() and isinstance(router_logits, torch.Tensor) and router_logits.requires_grad:
         return _BalanceLoss.apply(router_logits, expert_idx, score, valid, offsets)
     b, kept = _balance_args(router_logits, expert_idx, score, valid, offsets)

@@ -1,6 +1,7 @@
 """Host side of the training losses, without a GPU: which buffers the forms share, which calls are refused."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from lpmm import functional as F
 from lpmm import losses as L
@@ -37,3 +38,23 @@ def test_returned_counts_keep_no_workspace(host):
         counts = call(x, idx)[1]
         assert counts.untyped_storage().nbytes() == 64
         assert host.pop()[1].counts_out == counts.data_ptr()
+
+
+@pytest.mark.parametrize("name", ["logits", "teacher_logits", "weights", "router_logits"])
+@pytest.mark.parametrize("grad_mode", [True, False])
+@pytest.mark.parametrize("leaf", [False, True])
+def test_tensors_with_a_forward_tangent_are_refused(host, name, grad_mode, leaf):
+    kw = dict(logits=torch.randn(3, 10), teacher_logits=torch.randn(3, 2), teacher_idx=torch.zeros(3, 2, dtype=torch.int64),
+              weights=torch.ones(3))
+    call = F.topk_distillation
+    if name == "router_logits":
+        call, kw = F.balance_loss, dict(router_logits=torch.randn(3, 10), expert_idx=torch.zeros(3, 2, dtype=torch.int64))
+    if leaf:
+        kw["logits" if name != "router_logits" else name].requires_grad_()
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        dual = dict(kw, **{name: forward_ad.make_dual(kw[name], torch.ones_like(kw[name]))})
+        with pytest.raises(RuntimeError, match=f"{name} carries a forward-mode tangent"):
+            call(**dual)
+        assert not host, "nothing may be launched"
+        call(**kw)  # without a tangent it is an ordinary call
+        assert len(host) == 1
