@@ -1184,7 +1184,8 @@ static int distill_check(const lpmm_b200_distill* d, int mode) {
   if (d->rows && (!d->logits || !d->teacher || !d->index || !d->work)) return LPMM_B200_ERR_NULL_POINTER;
   if (d->rows && mode != DISTILL_LOSS && !d->grad) return LPMM_B200_ERR_NULL_POINTER;
   if (mode != DISTILL_GRAD && !d->loss && (d->rows || d->reduction != LPMM_B200_REDUCE_NONE)) return LPMM_B200_ERR_NULL_POINTER;
-  if (mode == DISTILL_GRAD && !d->upstream) return LPMM_B200_ERR_NULL_POINTER;
+  // without rows there are no values of REDUCE_NONE either, neither losses nor their derivatives
+  if (mode == DISTILL_GRAD && !d->upstream && (d->rows || d->reduction != LPMM_B200_REDUCE_NONE)) return LPMM_B200_ERR_NULL_POINTER;
   if ((uintptr_t)d->work & 15) return LPMM_B200_ERR_BAD_SIZE;
   if (d->rows && mode != DISTILL_LOSS) {  // 16-byte accesses follow both
     const int64_t size = d->dtype == LPMM_B200_DTYPE_FP32 ? 4 : 2;

@@ -3,6 +3,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from lpmm import _native as N
 from lpmm import functional as F
 from lpmm import losses as L
 
@@ -58,3 +59,22 @@ def test_tensors_with_a_forward_tangent_are_refused(host, name, grad_mode, leaf)
         assert not host, "nothing may be launched"
         call(**kw)  # without a tangent it is an ordinary call
         assert len(host) == 1
+
+
+@pytest.mark.parametrize("reduction", ["none", "sum", "mean"])
+@pytest.mark.parametrize("shape", [(0, 10), (2, 0, 10)])
+def test_backward_of_no_rows(monkeypatch, reduction, shape):
+    """Through the library's own checks; without rows the backward pass launches nothing."""
+    monkeypatch.setattr(L, "_check_cuda", lambda t, name: None)
+    status = []
+
+    def launch(fn, args, device):
+        if fn is N.lib.lpmm_b200_distill_backward:
+            status.append(fn(args, None))
+            N.check(status[-1])
+    monkeypatch.setattr(L, "_launch", launch)
+    x = torch.randn(shape, requires_grad=True)
+    t, idx = torch.zeros(*shape[:-1], 2), torch.zeros(*shape[:-1], 2, dtype=torch.int64)
+    loss = F.topk_distillation(x, t, idx, reduction=reduction)
+    (grad,) = torch.autograd.grad(loss.sum(), x)
+    assert grad.shape == shape and status == [0]
