@@ -439,18 +439,22 @@ __device__ __forceinline__ void prefetch_entries(const DistillArgs& a, long long
   for (int at = lane * 128; at < a.k * size; at += 32 * 128) prefetch_l2(t + at);
 }
 
-// 1 / sum of the weights (0 if that is 0) by a warp: at most OWN_NORM_ROWS of them, a few loads per lane
+// Sum of at most OWN_NORM_ROWS weights by a warp, a few loads per lane.  In double and always in this order: the kernels' factor
+// of the gradient and the sum over the rows' losses are then of the same number, also where weights of both signs cancel.
 constexpr int OWN_NORM_ROWS = 256;
-__device__ __forceinline__ float own_norm(const DistillArgs& a) {
-  float w = 0.0f;
+__device__ __forceinline__ double sum_of_few(const float* weights, long long rows) {
+  double w = 0.0;
 #pragma unroll
   for (int i = 0; i < OWN_NORM_ROWS; i += 32) {
     const int r = i + (threadIdx.x & 31);
-    if (r < a.rows) w += a.weights[r];
+    if (r < rows) w += weights[r];
   }
-  w = Warp().sum(w);
-  return w == 0.0f ? 0.0f : 1.0f / w;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(~0u, w, d);
+  return w;
 }
+__device__ __forceinline__ double norm_of(double w) { return w == 0.0 ? 0.0 : 1.0 / w; }
+__device__ __forceinline__ float own_norm(const DistillArgs& a) { return (float)norm_of(sum_of_few(a.weights, a.rows)); }
 
 // The gradient's factor that all rows share.  For whole warps: own_norm adds up over the lanes.
 __device__ __forceinline__ float shared_factor(const DistillArgs& a) {
@@ -1150,11 +1154,14 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
   __shared__ double red[2][32];
   pdl_start_next();
   pdl_wait();
+  const bool few = rows <= OWN_NORM_ROWS, weighted = mean && weights;
   double l = 0.0, w = 0.0;
   for (long long i = threadIdx.x; i < rows; i += blockDim.x) {
     if (row_loss) l += row_loss[i];
-    if (mean && weights) w += weights[i];
+    if (weighted && !few) w += weights[i];
   }
+  double all = 0.0;
+  if (weighted && few && threadIdx.x < 32) all = sum_of_few(weights, rows);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     l += __shfl_xor_sync(~0u, l, o);
@@ -1165,8 +1172,9 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
   if (threadIdx.x == 0) {
     l = w = 0.0;
     for (int i = 0; i < (int)(blockDim.x >> 5); ++i) l += red[0][i], w += red[1][i];
+    if (weighted && few) w = all;
     if (mean && !weights) w = (double)rows;
-    const double n = !mean ? 1.0 : w == 0.0 ? 0.0 : 1.0 / w;
+    const double n = !mean ? 1.0 : norm_of(w);
     if (norm) *norm = (float)n;
     if (loss) *loss = n == 0.0 ? 0.0f : (float)(l * n);
   }

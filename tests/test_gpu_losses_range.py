@@ -7,7 +7,8 @@ import torch
 
 from gpu_helpers import device
 from loss_ref import U32, balance_loss_bound
-from test_gpu_losses import DT, F, INF, REGIMES, balance_inputs, check_distill_copies, close, distill_inputs, same_bits
+from test_gpu_losses import (DT, F, INF, REGIMES, balance_inputs, check_distill, check_distill_copies, close, distill_inputs,
+                             same_bits)
 
 pytestmark = pytest.mark.gpu
 
@@ -131,6 +132,20 @@ def test_balance_loss_of_many_tokens(tokens, cuts, score):
     c = counts.double().cpu().view(-1, 248)
     ref = (248 * c / c.sum(1, keepdim=True) * p).sum(1).view(loss.shape)
     close(loss, ref, balance_loss_bound(ref, 0, 248))  # its constant part has the 512 additions of a run
+
+
+# ----------------------------------------------------------------------------------------------
+# weights that cancel
+# ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [4, 40, 160, 256, 258])
+@pytest.mark.parametrize("vocab", [700, 10000, 40000])
+def test_distillation_mean_over_weights_that_cancel(rows, vocab):
+    """Their sum is 1.5 and exact in double, in any order; in fp32 it would be 0: loss and gradient have the same mean."""
+    x, t, idx = distill_inputs(rows, vocab, 5, "bf16", seed=28)
+    w = torch.tensor([3.0, -3.0]).repeat(rows // 2)
+    w[:4] = torch.tensor([2.0 ** 25, -2.0 ** 25, 1.0, 0.5])
+    assert w.double().sum() == 1.5
+    check_distill(x, t, idx, 2.0, w.to(device()), "mean")
 
 
 # ----------------------------------------------------------------------------------------------
