@@ -6,6 +6,8 @@ Each comes as a differentiable function and as a ``..._with_grad`` form that ret
 the logits are then read once instead of twice, and nothing of autograd runs.  Both launch on torch's current stream
 of the logits' device and synchronise nothing.
 """
+import functools
+
 import torch
 from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
@@ -33,10 +35,12 @@ def _check_tensor(t, name, dtypes, like):
         raise RuntimeError(f"The type of {name} is not correct: {t.dtype}")
 
 
+# -1 while no forward-mode level is open: there are no dual tensors then
+_dual_level = (lambda: forward_ad._current_level) if hasattr(forward_ad, "_current_level") else (lambda: 0)
+
+
 def _refuse_tangents(tensors):
     """The differentiable forms have no forward-mode derivative: a dual tensor would lose its tangent in silence."""
-    if getattr(forward_ad, "_current_level", 0) < 0:  # no level is open, so there are no dual tensors
-        return
     for t, name in tensors:
         if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
             raise RuntimeError(f"{name} carries a forward-mode tangent, which is not supported: only the backward pass is")
@@ -193,7 +197,8 @@ def topk_distillation(logits, teacher_logits, teacher_idx, temperature=1.0, weig
 
     An index of V or more makes its row's loss and gradient NaN.  Results do not depend on scheduling.  Tensors with
     forward-mode tangents are refused."""
-    _refuse_tangents(((logits, "logits"), (teacher_logits, "teacher_logits"), (weights, "weights")))
+    if _dual_level() >= 0:
+        _refuse_tangents(((logits, "logits"), (teacher_logits, "teacher_logits"), (weights, "weights")))
     if torch.is_grad_enabled():
         for t, name in ((teacher_logits, "teacher_logits"), (weights, "weights")):
             if isinstance(t, torch.Tensor) and t.requires_grad:
@@ -260,14 +265,20 @@ def _balance_args(router_logits, expert_idx, score, valid, offsets):
     return b, (logits, idx, valid, offsets)
 
 
+@functools.lru_cache(maxsize=64)
+def _balance_work_bytes(experts, sequences):
+    nbytes = N.lib.lpmm_b200_balance_work_bytes(experts, sequences)  # a multiple of 16
+    if nbytes < 0:
+        N.check(int(nbytes))
+    return nbytes
+
+
 def _balance_outputs(b, device):
     """Loss, counts, and the buffer that holds what belongs to the call: counts that the backward pass reads (the caller may do
     with the returned ones as it likes), the workspace behind them and the gradient's factors."""
     s, e = b.sequences, b.experts
     cells = s * e
-    nbytes = N.lib.lpmm_b200_balance_work_bytes(e, s)  # a multiple of 16
-    if nbytes < 0:
-        N.check(int(nbytes))
+    nbytes = _balance_work_bytes(e, s)
     buf = torch.empty(cells + nbytes // 8 + (s + 1) // 2, dtype=torch.int64, device=device)
     loss = torch.empty((s,) if b.offsets else (), dtype=torch.float32, device=device)
     at = buf.data_ptr()
@@ -317,7 +328,8 @@ def balance_loss(router_logits, expert_idx, score="softmax", valid=None, offsets
 
     An index of E or more makes its sequence's loss and gradient NaN, offsets that descend or leave the range make every
     loss NaN.  Results do not depend on scheduling.  Logits with a forward-mode tangent are refused."""
-    _refuse_tangents(((router_logits, "router_logits"),))
+    if _dual_level() >= 0:
+        _refuse_tangents(((router_logits, "router_logits"),))
     if torch.is_grad_enabled() and isinstance(router_logits, torch.Tensor) and router_logits.requires_grad:
         return _BalanceLoss.apply(router_logits, expert_idx, score, valid, offsets)
     b, kept = _balance_args(router_logits, expert_idx, score, valid, offsets)
