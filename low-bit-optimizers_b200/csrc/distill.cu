@@ -540,7 +540,8 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
   const float up0 = MODE == DISTILL_LOSS ? 0.0f : shared_factor(a);
   int st = 0, it = 0;
   uint32_t phase = 0;
-  for (long long row = row0; row < rows; ++it, row += stride) {
+  long long row = row0;
+  for (; row < rows; ++it, row += stride) {
     const RowFetch<T, MODE, KV> f = next;
     next.load(a, row + stride);
     const T* x = logits_row<T>(a, row);
@@ -549,7 +550,7 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
     char* slot = slots + st * a.slot;
     const T* xs = reinterpret_cast<const T*>(slot);  // column `head` is its first
     const uint4* buf = reinterpret_cast<const uint4*>(slot);
-    mbar_wait(&full[warp][st], phase, &failed);
+    if (!__all_sync(~0u, mbar_wait(&full[warp][st], phase, &failed))) break;
 
     // entries
     int idx[KV];
@@ -703,9 +704,14 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
     copy(row + (long long)a.stages * stride, st, (ahead < 32 ? dead >> ahead : dead_next >> (ahead - 32)) & 1);
     if (++st == a.stages) st = 0, phase ^= 1;
   }
+  if (lane == 0)  // only where a wait ran out: the copies under way, of this row and the next ones, still have to land
+    for (int i = 0; i < a.stages && row + (long long)i * stride < rows; ++i) {
+      mbar_wait_landed(&full[warp][st], phase);
+      if (++st == a.stages) st = 0, phase ^= 1;
+    }
   __syncthreads();
   if (failed)  // a wait ran out (it never has): what this CTA wrote is not to be taken for a result
-    for (long long row = row0; row < rows; row += stride)
+    for (row = row0; row < rows; row += stride)
       if (lane == 0) {
         if (MODE != DISTILL_GRAD) a.row_loss[row] = nan_f();
         if (MODE != DISTILL_LOSS) grad_row<T>(a, row)[0] = E::narrow(nan_f());
@@ -978,8 +984,10 @@ __global__ void __launch_bounds__(32 * (CW + 1 + Shape<MODE, CW>::TELLERS), Shap
             // every part sends its statistics to all.  Two sets in turn: a part sends for row n + 2 after it has all of
             // row n + 1, that is after every part has read row n's.
             const int set = joins & 1;
-            if (tid == 0) mbar_expect(&sm.joined[set], parts * (uint32_t)sizeof(float2));
-            if (tid < parts) send_async(&sm.part[set][part], make_float2(r.m, r.s), &sm.joined[set], tid);
+            if (!*(volatile int*)&sm.failed) {  // a barrier whose phase did not come is not armed again
+              if (tid == 0) mbar_expect(&sm.joined[set], parts * (uint32_t)sizeof(float2));
+              if (tid < parts) send_async(&sm.part[set][part], make_float2(r.m, r.s), &sm.joined[set], tid);
+            }
             mbar_wait_cluster(&sm.joined[set], joins >> 1 & 1, &sm.failed);
             ++joins;
             r = Consumers<CW>::join_of(sm.part[set][lane % parts], parts, a.c);

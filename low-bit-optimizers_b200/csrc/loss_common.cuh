@@ -161,14 +161,17 @@ __device__ __forceinline__ bool mbar_test_cluster(unsigned long long* b, uint32_
       : "memory");
   return done;
 }
-// Waits for the phase; gives up when the limit is reached or another thread of the CTA has given up (*failed).  The
-// caller goes on in either case (its data are then worthless, its accesses in range) and the kernel ends as it should.
-__device__ __forceinline__ void mbar_wait(unsigned long long* b, uint32_t parity, int* failed) {
-  if (mbar_test(b, parity)) return;
+// Waits for the phase; gives up (false) when the limit is reached or another thread of the CTA has given up (*failed).  The
+// caller goes on in either case (its data are then worthless, its accesses in range) but starts no more copies, waits for those
+// under way, and the kernel ends as it should.
+__device__ __forceinline__ bool mbar_wait(unsigned long long* b, uint32_t parity, int* failed) {
+  if (mbar_test(b, parity)) return true;
   for (int i = 0; i < WAIT_LIMIT; ++i) {
-    if (mbar_test(b, parity) || *(volatile int*)failed) return;
+    if (mbar_test(b, parity)) return true;
+    if (*(volatile int*)failed) return false;
   }
   *(volatile int*)failed = 1;
+  return false;
 }
 // the same for data that other CTAs of the cluster send
 __device__ __forceinline__ void mbar_wait_cluster(unsigned long long* b, uint32_t parity, int* failed) {
