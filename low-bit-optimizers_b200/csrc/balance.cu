@@ -8,7 +8,8 @@
 // indices are counted.  A token's logits lie in the registers of up to 32 lanes, some tokens per warp at a time; a warp
 // walks a contiguous run of tokens and sums the scores of its columns in registers, in fp32.  Those sums (of MAX_RUN tokens at
 // most, so that their rounding does not grow with the batch) meet as 64-bit whole numbers, in units of 2^-shift with tokens * 2^shift < 2^62: atomics on
-// them give the same result in any order, and what is rounded off is far below fp32 of the sum.
+// them give the same result in any order, and what is rounded off is far below fp32 of the scores' sum (of the loss, whose
+// usual size is 1, at most experts * tokens * 2^-62).
 // Bound by memory for large batches (a logit is read once, a gradient written once), by launches for small ones: these
 // are done in one launch of a CTA or a cluster, larger ones in three (clear, count, scores; the last CTA adds up).
 #include <cooperative_groups.h>

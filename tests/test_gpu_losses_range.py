@@ -7,7 +7,7 @@ import torch
 
 from gpu_helpers import device
 from loss_ref import U32, balance_loss_bound
-from test_gpu_losses import (DT, F, INF, REGIMES, balance_inputs, check_distill, check_distill_copies, close, distill_inputs,
+from test_gpu_losses import (DT, F, INF, REGIMES, balance_inputs, check_balance, check_distill, check_distill_copies, close, distill_inputs,
                              same_bits)
 
 pytestmark = pytest.mark.gpu
@@ -179,3 +179,75 @@ def test_distillation_from_two_threads(sizes):
     for t in threads:
         t.join()
     assert not errors, errors
+
+
+# ----------------------------------------------------------------------------------------------
+# captured passes of every size
+# ----------------------------------------------------------------------------------------------
+def captured(step):
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = [v.clone() for v in step()]
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    return graph, want, got
+
+
+def check_replays(step, x, other):
+    """A replay has the bits of the ordinary call, twice, and those of the other inputs once they lie in the same memory."""
+    graph, want, got = captured(step)
+    for _ in range(2):
+        for v in got:
+            v.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(same_bits(a, b) for a, b in zip(want, got))
+    with torch.no_grad():
+        x.copy_(other)
+    want = [v.clone() for v in step()]
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(same_bits(a, b) for a, b in zip(want, got))
+
+
+# rows of their own, a ring of each size, clusters, few rows; the sum of the weights inside the kernel and before it
+@pytest.mark.parametrize("rows, vocab", [(300, 700), (200, 12000), (300, 12000), (300, 40000), (160, 131072), (300, 131072), (7, 50257)])
+def test_distillation_captured(rows, vocab):
+    x, t, idx = distill_inputs(rows, vocab, 9, "bf16", seed=29)
+    w = torch.rand(rows, generator=torch.Generator().manual_seed(30)).to(device())
+    check_replays(lambda: F().topk_distillation_with_grad(x, t, idx, 2.0, w), x, x * 0.5)
+    x.requires_grad_()
+
+    def train():
+        loss = F().topk_distillation(x, t, idx, 2.0, w)
+        return loss.detach(), torch.autograd.grad(loss, x)[0]
+    check_replays(train, x, x.detach() * 0.5)
+
+
+@pytest.mark.parametrize("tokens, experts, sequences", [(48, 8, 0), (3000, 64, 5), (30000, 64, 0), (30000, 64, 100)])
+def test_balance_captured(tokens, experts, sequences):
+    x, idx = balance_inputs(tokens, experts, 2, "bf16", seed=31)
+    offsets = torch.linspace(0, tokens, sequences + 1, device=device()).long() if sequences else None
+    check_replays(lambda: F().balance_loss_with_grad(x, idx, offsets=offsets), x, x * 0.5)
+    x.requires_grad_()
+
+    def train():
+        loss, counts = F().balance_loss(x, idx, offsets=offsets)
+        return loss.detach(), counts, torch.autograd.grad(loss.sum(), x)[0]
+    check_replays(train, x, x.detach() * 0.5)
+
+
+# ----------------------------------------------------------------------------------------------
+# many experts per token
+# ----------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens, experts, k", [(70, 2, 5), (100, 33, 33), (45, 700, 500), (1000, 64, 1024), (3000, 100, 31)])
+def test_balance_many_chosen(tokens, experts, k):
+    g = torch.Generator().manual_seed(32)
+    x = torch.randn(tokens, experts, generator=g).to(device())
+    idx = torch.randint(-1, experts, (tokens, k), generator=g).int().to(device())
+    valid = (torch.rand(tokens, generator=g) < 0.8).to(device())
+    check_balance(x, idx, "softmax", valid, torch.tensor([0, tokens // 3, tokens], device=device()), grad_scale=float(tokens))
+    check_balance(x, idx, "sigmoid", None, None, grad_scale=float(tokens))
