@@ -423,11 +423,19 @@ __device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int 
   for (int s = one ? 0 : first + warp; s < a.sequences; s += step) {
     double sum = 0.0;
     const int from = one ? threadIdx.x : lane, by = one ? blockDim.x : 32;
-#pragma unroll 4
-    for (int e = from; e < a.experts; e += by) {
-      const unsigned long long c = __ldcg(&a.counts[cell(a, s, e)]);
-      sum += (double)c * (double)__ldcg(&a.psum[cell(a, s, e)]);
-      if (a.counts_out) a.counts_out[cell(a, s, e)] = c;
+    for (int e0 = from; e0 < a.experts; e0 += 4 * by) {  // four at a time: their loads first, which a store would hold up
+      unsigned long long c[4], p[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int e = e0 + j * by;
+        c[j] = e < a.experts ? __ldcg(&a.counts[cell(a, s, e)]) : 0;
+        p[j] = e < a.experts ? __ldcg(&a.psum[cell(a, s, e)]) : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        sum += (double)c[j] * (double)p[j];
+        if (a.counts_out && e0 + j * by < a.experts) a.counts_out[cell(a, s, e0 + j * by)] = c[j];
+      }
     }
     const double f = factor_of(a, s);
     const int nan = __ldcg(&a.bad[s]) & 2;
