@@ -439,26 +439,44 @@ __device__ __forceinline__ void prefetch_entries(const DistillArgs& a, long long
   for (int at = lane * 128; at < a.k * size; at += 32 * 128) prefetch_l2(t + at);
 }
 
-// Sum of at most OWN_NORM_ROWS weights by a warp, a few loads per lane.  In double and always in this order: the kernels' factor
-// of the gradient and the sum over the rows' losses are then of the same number, also where weights of both signs cancel.
+// The gradient's factor that all rows share, for whole warps.  With few rows its norm is 1 / sum of the weights (0 if that is
+// 0), added up here: in double and in the order of distill_reduce_kernel (32 rows by a tree, these sums one after another), so
+// that gradient and loss are means over the same number, also where weights of both signs cancel.  `load` and `get` lie apart
+// where there is work to do in between.
 constexpr int OWN_NORM_ROWS = 256;
-__device__ __forceinline__ double sum_of_few(const float* weights, long long rows) {
-  double w = 0.0;
+__device__ __noinline__ float far_reciprocal(double w) { return w == 0.0 ? 0.0f : (float)(1.0 / w); }
+struct SharedFactor {
+  float v[OWN_NORM_ROWS / 32], norm;
+  __device__ __forceinline__ void load(const DistillArgs& a) {
+    norm = a.norm ? *a.norm : 1.0f;
 #pragma unroll
-  for (int i = 0; i < OWN_NORM_ROWS; i += 32) {
-    const int r = i + (threadIdx.x & 31);
-    if (r < rows) w += weights[r];
+    for (int i = 0; i < OWN_NORM_ROWS / 32; ++i) {
+      const int r = i * 32 + (threadIdx.x & 31);
+      v[i] = a.own_norm && r < a.rows ? a.weights[r] : 0.0f;
+    }
   }
+  __device__ __forceinline__ float get(const DistillArgs& a) const {
+    float n = norm;
+    if (a.own_norm) {
+      double w = 0.0;
 #pragma unroll
-  for (int d = 16; d; d >>= 1) w += __shfl_xor_sync(~0u, w, d);
-  return w;
-}
-__device__ __forceinline__ double norm_of(double w) { return w == 0.0 ? 0.0 : 1.0 / w; }
-__device__ __forceinline__ float own_norm(const DistillArgs& a) { return (float)norm_of(sum_of_few(a.weights, a.rows)); }
-
-// The gradient's factor that all rows share.  For whole warps: own_norm adds up over the lanes.
+      for (int i = 0; i < OWN_NORM_ROWS / 32; ++i) {
+        if (i * 32 >= a.rows) break;
+        double t = v[i];
+#pragma unroll
+        for (int d = 16; d; d >>= 1) t += __shfl_xor_sync(~0u, t, d);
+        w += t;
+      }
+      const float f = (float)w;  // an fp32 division is off by one rounding more than one in double and much shorter
+      n = fabsf(f) > 1e-30f && fabsf(f) < 1e30f ? 1.0f / f : far_reciprocal(w);
+    }
+    return a.scale * a.temperature * n;
+  }
+};
 __device__ __forceinline__ float shared_factor(const DistillArgs& a) {
-  return a.scale * a.temperature * (a.norm ? *a.norm : a.own_norm ? own_norm(a) : 1.0f);
+  SharedFactor f;
+  f.load(a);
+  return f.get(a);
 }
 __device__ __forceinline__ float upstream_of(const DistillArgs& a, long long row) {
   return a.upstream ? a.upstream[a.upstream_per_row ? row : 0] : 1.0f;
@@ -1102,6 +1120,8 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
     }
     return;
   }
+  SharedFactor factor;
+  if (MODE != DISTILL_LOSS) factor.load(a);
   if (MODE != DISTILL_GRAD) {
     // one pass over the row: running maximum and sum
     const Span o = span_of(x, lo, hi);
@@ -1140,7 +1160,7 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
     }
   }
   if (MODE == DISTILL_LOSS) return;
-  const float G = shared_factor(a) * upstream_of(a, row) * t.w + (t.ts - t.ts);  // NaN for a row with invalid entries
+  const float G = factor.get(a) * upstream_of(a, row) * t.w + (t.ts - t.ts);  // NaN for a row with invalid entries
   const float gs = G * rcp_nr(st.s);
   if (mark_entries(a, e, team, marks, lo, hi)) twice = 1;
   {
@@ -1162,14 +1182,11 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
   __shared__ double red[2][32];
   pdl_start_next();
   pdl_wait();
-  const bool few = rows <= OWN_NORM_ROWS, weighted = mean && weights;
   double l = 0.0, w = 0.0;
   for (long long i = threadIdx.x; i < rows; i += blockDim.x) {
     if (row_loss) l += row_loss[i];
-    if (weighted && !few) w += weights[i];
+    if (mean && weights) w += weights[i];
   }
-  double all = 0.0;
-  if (weighted && few && threadIdx.x < 32) all = sum_of_few(weights, rows);
 #pragma unroll
   for (int o = 16; o; o >>= 1) {
     l += __shfl_xor_sync(~0u, l, o);
@@ -1180,9 +1197,8 @@ __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __res
   if (threadIdx.x == 0) {
     l = w = 0.0;
     for (int i = 0; i < (int)(blockDim.x >> 5); ++i) l += red[0][i], w += red[1][i];
-    if (weighted && few) w = all;
     if (mean && !weights) w = (double)rows;
-    const double n = !mean ? 1.0 : norm_of(w);
+    const double n = !mean ? 1.0 : w == 0.0 ? 0.0 : 1.0 / w;
     if (norm) *norm = (float)n;
     if (loss) *loss = n == 0.0 ? 0.0f : (float)(l * n);
   }
