@@ -462,8 +462,10 @@ __global__ void __launch_bounds__(1024) balance_count_kernel(const BalanceArgs a
   count_phase(a, offsets, blockIdx.x, reinterpret_cast<int*>(shared));
 }
 
-// Two CTAs per SM, so that four tokens per group of lanes and the next four fit in registers (131072 x 256 bf16, both: 46 us;
-// three CTAs 55, two tokens 51).  Bound by issue: 190 instructions per warp and token, 64 % of the slots.
+// Two CTAs per SM, so that four tokens per group of lanes and the next four fit in registers (131072 x 256 bf16, both: 46-50 us;
+// three CTAs 55, two tokens 51).  Bound by issue: 190 instructions per warp and token, 64 % of the slots.  With the gradient,
+// more than 512 experts spill (80-700 bytes, single loads up to 944; the traffic stays on the chip): 32768 x 1024 bf16 62 us
+// a call, 0.33 of the copy rate, fp32 76 us, 0.54; 32768 x 1023 bf16 139 us, 0.15.
 template <typename T, int V, int J, bool SIG, bool SUM, bool GRAD>
 __global__ void __launch_bounds__(256, 2) balance_score_kernel(const BalanceArgs a) {
   extern __shared__ unsigned long long shared[];
@@ -492,7 +494,8 @@ __global__ void __launch_bounds__(256) balance_loss_kernel(const BalanceArgs a) 
 }
 
 // Everything in one launch of one cluster (of one CTA, where that is enough).  Bound by latencies: four phases with a barrier
-// of the cluster between them, 10-14 us (4096 x 64 bf16: 14 us; the three launches take 16.6 us at 16384 x 64).
+// of the cluster between them, 11-17 us (1024 x 64 bf16: 14 us, 4096 x 64: 16.5 us, as much
+// as the three launches take at 16384 x 64).
 template <typename T, int V, int J, int U, bool SIG, bool GRAD>
 __global__ void __launch_bounds__(MAX_WARPS * 32, 1) balance_small_kernel(const BalanceArgs a) {
   extern __shared__ unsigned long long shared[];

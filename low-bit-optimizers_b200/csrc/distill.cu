@@ -494,7 +494,7 @@ __device__ __noinline__ float far_sum(const DistillArgs& a, const T* x, int lo, 
 // rows: every warp takes rows of its own; their logits are copied into its slots of shared memory some rows ahead, the
 // entries of the next row are loaded into registers (KV per lane).  A warp needs no barrier with others, and a gathered logit
 // comes from shared memory.  Bound by instructions: about 900 per row and warp beside its columns (loss and gradient of
-// 512 MB of bf16 logits, 64 entries: 4096 columns 311 us = 0.53 of the copy rate, 1000 columns 421 us = 0.42).
+// 512 MB of bf16 logits, 64 entries: 4096 columns 316 us = 0.53 of the copy rate, 1000 columns 426 us = 0.42).
 // ---------------------------------------------------------------------------------------------
 constexpr int ROWS_MAX_WARPS = 8, ROWS_MAX_STAGES = 4, ROWS_MAX_BYTES = 16384;
 constexpr size_t rows_room(int ctas) { return 227 * 1024 / ctas - 2048; }  // shared memory of a CTA
@@ -742,7 +742,7 @@ __global__ void __launch_bounds__(ROWS_MAX_WARPS * 32, KV <= 2 ? 3 : 2) distill_
 // softmax and the losses, a chain of latencies per row, are thus off the path that the row's columns take.
 // Bound by memory and, for 16-bit types, by how many chunks' latencies four warps per scheduler hide (the pipe of the
 // exponentials is 54-65 % busy).  512 MB of logits, 64 entries: loss, bf16, 32000 columns 106 us = 0.78 of the copy rate
-// (fp32 96 us, 0.85); gradient 207 us, 0.79; both 226 us, 0.73 (fp32 207 us, 0.79).
+// (fp32 97 us, 0.84); gradient 213 us, 0.77; both 225 us, 0.73 (fp32 206 us, 0.79).
 // ---------------------------------------------------------------------------------------------
 constexpr int PER = 4;  // vectors per consuming thread and chunk
 constexpr int MAX_STAGES = 14, MAX_TELLERS = 4, MAX_PARTS = 8;
@@ -1175,7 +1175,8 @@ __global__ void __launch_bounds__(512) distill_split_kernel(const DistillArgs a)
   write_entries(a, g, e, team, marks, twice != 0, ex, gs, G, t.ts, lo, hi);
 }
 
-// One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double (3 us).
+// One CTA: the sum of the weights and of the weighted row losses in a fixed order, in double (3 us up to some
+// thousand rows, 5 us at 16384, 12 at 67108, 40 at 268435).
 __global__ void __launch_bounds__(1024) distill_reduce_kernel(const float* __restrict__ row_loss,
                                                               const float* __restrict__ weights, long long rows, int mean,
                                                               float* __restrict__ loss, float* __restrict__ norm) {
