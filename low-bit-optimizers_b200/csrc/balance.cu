@@ -7,9 +7,9 @@
 // The gradient needs the counts, not the summed scores, so loss and gradient share one pass over the logits once the
 // indices are counted.  A token's logits lie in the registers of up to 32 lanes, some tokens per warp at a time; a warp
 // walks a contiguous run of tokens and sums the scores of its columns in registers, in fp32.  Those sums (of MAX_RUN tokens at
-// most, so that their rounding does not grow with the batch) meet as 64-bit whole numbers, in units of 2^-shift with tokens * 2^shift < 2^62: atomics on
-// them give the same result in any order, and what is rounded off is far below fp32 of the scores' sum (of the loss, whose
-// usual size is 1, at most experts * tokens * 2^-62).
+// most, so that their rounding does not grow with the batch) meet as 64-bit whole numbers, in units of 2^-shift with
+// tokens * 2^shift < 2^62: atomics on them give the same result in any order, and what is rounded off is far below fp32 of the
+// scores' sum (of the loss, whose usual size is 1, at most experts * tokens * 2^-62).
 // Bound by memory for large batches (a logit is read once, a gradient written once), by launches for small ones: these
 // are done in one launch of a CTA or a cluster, larger ones in three (clear, count, scores; the last CTA adds up).
 #include <cooperative_groups.h>
@@ -415,8 +415,8 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// Loss and factor of the sequences, and the second copy of their counts.  Reads what other CTAs have written; the loads of a thread are independent of one
-// another.  A sequence has a warp, or, where there is one sequence only, the CTA (`red`: double[32]).
+// Loss and factor of the sequences, and the second copy of their counts.  Reads what other CTAs have written; the loads of a
+// thread are independent of one another.  A sequence has a warp, or, where there is one sequence only, the CTA (`red`: double[32]).
 __device__ __forceinline__ void loss_phase(const BalanceArgs& a, int first, int step, double* red) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool one = a.sequences == 1;

@@ -324,7 +324,8 @@ def balance_loss(router_logits, expert_idx, score="softmax", valid=None, offsets
     valid takes no part and has gradient 0 whatever its logits hold.  ``offsets``: int32 or int64 ``[S + 1]``, ascending:
     sequence s is the flattened tokens ``offsets[s]`` to ``offsets[s + 1]``, with a loss and counts of its own (``[S]``
     and ``[S, E]``, else scalar and ``[E]``); tokens outside of all sequences take no part, a sequence without valid
-    tokens has loss 0.  Loss fp32, counts int64, gradient of the logits' type, rounded once.
+    tokens has loss 0.  Loss fp32, counts int64 (the caller's own: nothing reads them later), gradient of the logits'
+    type, rounded once.
 
     An index of E or more makes its sequence's loss and gradient NaN, offsets that descend or leave the range make every
     loss NaN.  Results do not depend on scheduling.  Logits with a forward-mode tangent are refused."""
